@@ -39,6 +39,15 @@ static inline int uem_flat_grid(int64_t work_items, int block) {
     return uem_stream_grid(work_items, block);
 }
 
+// Clears n 4-byte words on the stream.  A kernel and not hipMemsetAsync: the callers may be captured into a hipGraph, and memset nodes
+// have given wrong results on replays after the first.
+static __global__ __launch_bounds__(256) void clear_words_kernel(uint32_t* __restrict__ p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0u;
+}
+static inline void uem_clear_words(void* p, int64_t n, hipStream_t st) {
+    clear_words_kernel<<<uem_stream_grid(n, 256), 256, 0, st>>>((uint32_t*)p, n);
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

@@ -289,7 +289,7 @@ __global__ void index_max_kernel(const int64_t* __restrict__ idx, int64_t count,
 extern "C" int uem_index_max(const int64_t* idx, int64_t count, int64_t* out, void* stream) {
     UEM_REQUIRE(idx && out && count > 0, "index_max: bad arguments");
     hipStream_t st = (hipStream_t)stream;
-    hipMemsetAsync(out, 0, sizeof(int64_t), st);
+    uem_clear_words(out, 2, st);
     index_max_kernel<<<uem_stream_grid(count, 256 * 4), 256, 0, st>>>(idx, count, (unsigned long long*)out);
     return uem_check_launch("index_max");
 }
@@ -868,7 +868,7 @@ __global__ void plane_max_decode_kernel(uint32_t* pm, int n) {
 extern "C" int uem_plane_max(const float* mask, uint32_t* plane_max, int B, int C, int64_t HW, void* stream) {
     UEM_REQUIRE(mask && plane_max && B > 0 && C > 0 && HW > 0, "plane_max: bad arguments");
     hipStream_t st = (hipStream_t)stream;
-    hipMemsetAsync(plane_max, 0, sizeof(uint32_t) * B * C, st);
+    uem_clear_words(plane_max, (int64_t)B * C, st);
     int chunks = (int)uem_cdiv(HW, 256 * 8);
     if (chunks > 64) chunks = 64;
     plane_max_kernel<<<dim3(chunks, B * C), 256, 0, st>>>(mask, plane_max, HW);
@@ -1071,8 +1071,8 @@ extern "C" int uem_scatter(const float* src, const int64_t* index, float* out, f
     UEM_REQUIRE(B > 0 && N > 0 && C > 0 && S > 0 && reduce >= 0 && reduce <= 2, "scatter: bad arguments");
     UEM_REQUIRE(reduce != 2 || workspace, "scatter: mean needs a B*S workspace");
     hipStream_t st = (hipStream_t)stream;
-    hipMemsetAsync(out, 0, sizeof(float) * (size_t)B * S * C, st);
-    if (reduce == 2) hipMemsetAsync(workspace, 0, sizeof(float) * (size_t)B * S, st);
+    uem_clear_words(out, (int64_t)B * S * C, st);
+    if (reduce == 2) uem_clear_words(workspace, (int64_t)B * S, st);
     scatter_kernel<<<dim3((unsigned)uem_cdiv(N, 256), (unsigned)B), 256, 0, st>>>(src, index, out, workspace, N, C, S, reduce);
     const int64_t total = (int64_t)B * S * C;
     if (reduce != 1) scatter_finish_kernel<<<(int)uem_cdiv(total, 256), 256, 0, st>>>(out, workspace, total, C, reduce);
