@@ -489,6 +489,19 @@ int uem_weight_prep_blocks(int kind, int cout, int cin, int taps);   /* blocks t
 int uem_weight_prep(const uem_prep_job* jobs /* device */, const int* block_starts /* device, njobs + 1 */, int njobs,
                     int total_blocks, void* stream);
 
+/* ---- layer normalisation over the channels of feature rows ------------------------------------------------------------------
+ * y = (x - mean) / sqrt(var + eps) * gamma + beta per row of C channels; x[rows][C] with a row stride of x_ld elements, y / dx dense.
+ * x, y, dy, dx share one type: fp32, or bf16 with UEM_LN_BF16; gamma / beta (either may be NULL: ones / zeros) and their gradients are
+ * fp32, or bf16 with UEM_LN_PARAM_BF16.  mean / rstd [rows] fp32: written by the forward (both NULL: not saved), read by the backward.
+ * Backward: dgamma / dbeta are WRITTEN (either may be NULL) and need the workspace; their sums run in a fixed order.             */
+#define UEM_LN_BF16 1
+#define UEM_LN_PARAM_BF16 2
+int64_t uem_layernorm_workspace_floats(int64_t rows, int C);
+int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma, const void* beta, void* y, float* mean, float* rstd, int64_t rows,
+                      int C, float eps, int flags, void* stream);
+int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const void* gamma, const float* mean, const float* rstd,
+                      void* dx, void* dgamma, void* dbeta, float* workspace, int64_t rows, int C, int flags, void* stream);
+
 /* ---- data parallel (new relative to the reference, which is single-GPU: SURVEY 2a, 8e) --------------------------
  * all-reduce(sum, in place) of a flat fp32 buffer -- the gradient arena, 98 MB for R50-ASPP -- over RCCL on `stream`:
  * one process per GPU, xGMI inside the node.  Rank 0 draws an id with uem_comm_unique_id, the host ships those 128

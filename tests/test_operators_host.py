@@ -1,0 +1,47 @@
+"""What the operators refuse, on the CPU: nothing here launches a kernel."""
+import pytest
+import torch
+
+from uemda_amd import _lib
+from uemda_amd._lib import UemError
+
+
+def test_layer_norm_refusals():
+    from uemda_amd.norm import LayerNorm, layer_norm
+    x = torch.zeros(4, 8)
+    with pytest.raises(UemError, match="MI355X"):
+        layer_norm(x)
+    with pytest.raises(UemError, match="float32 or bfloat16"):
+        layer_norm(x.half())
+    with pytest.raises(UemError, match="float32 or bfloat16"):
+        layer_norm([1.0])
+    with pytest.raises(UemError, match="channels"):
+        LayerNorm(0)
+    with pytest.raises(UemError, match="channel_dim"):
+        LayerNorm(8, channel_dim=2)
+    lib = _lib.load()
+    assert lib.uem_layernorm_fwd(None, 8, None, None, None, None, None, 4, 8, 1e-5, 0, None) == -1
+    assert lib.uem_layernorm_fwd(16, 7, None, None, 16, None, None, 4, 8, 1e-5, 0, None) == -1          # rows closer than their length
+    assert lib.uem_layernorm_fwd(16, 8, None, None, 16, 16, None, 4, 8, 1e-5, 0, None) == -1            # mean without rstd
+    assert lib.uem_layernorm_fwd(16, 8, None, None, 16, None, None, 0, 8, 1e-5, 0, None) == -1
+    assert lib.uem_layernorm_fwd(16, 8, None, None, 16, None, None, 4, 8, 1e-5, 64, None) == -1
+    assert lib.uem_layernorm_bwd(16, 8, 16, 8, None, 16, 16, 16, 16, None, None, 4, 8, 0, None) == -1     # gradients without a workspace
+    assert b"workspace" in lib.uem_last_error()
+    for rows, c in ((1, 5), (1000, 7), (10 ** 6, 256)):
+        assert lib.uem_layernorm_workspace_floats(rows, c) >= 2 * c
+
+
+def test_layer_norm_formula_against_differences():
+    """the 64-bit formulas that the device tests hold the kernels to are each other's derivatives"""
+    from test_gpu_layernorm import reference
+    g = torch.Generator().manual_seed(0)
+    x, w, b, dy = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((5, 7), (7,), (7,), (5, 7)))
+    _, dx, dw, db = reference(x, w, b, dy, 1e-5)[:4]
+    h = 1e-6
+    for t, grad in ((x, dx), (w, dw), (b, db)):
+        v = torch.randn(t.shape, generator=g, dtype=torch.float64)
+        t0 = t.clone()
+        t.copy_(t0 + h * v); up = (reference(x, w, b, dy, 1e-5)[0] * dy).sum()
+        t.copy_(t0 - h * v); down = (reference(x, w, b, dy, 1e-5)[0] * dy).sum()
+        t.copy_(t0)
+        assert abs((up - down) / (2 * h) - (grad * v).sum()) < 1e-7 * (1 + (grad * v).abs().sum())

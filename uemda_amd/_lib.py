@@ -144,6 +144,9 @@ SIGNATURES = {
     "uem_wino_filter_grad": [P, P, I, I, I, P],
     "uem_weight_prep_blocks": [I, I, I, I],
     "uem_weight_prep": [P, P, I, I, P],
+    "uem_layernorm_workspace_floats": [L, I],
+    "uem_layernorm_fwd": [P, L, P, P, P, P, P, L, I, F, I, P],
+    "uem_layernorm_bwd": [P, L, P, L, P, P, P, P, P, P, P, L, I, I, P],
     "uem_comm_unique_id": [P],
     "uem_comm_init": [POINTER(c_void_p), P, I, I],
     "uem_allreduce_flat": [P, P, L, P],
@@ -153,7 +156,7 @@ SIGNATURES = {
 }
 _RESTYPE = {"uem_last_error": c_char_p, "uem_bn_workspace_floats": c_int64,
             "uem_label_refine_workspace_floats": c_int64, "uem_label_refine_select_workspace_bytes": c_int64, "uem_stem_conv_wgrad_workspace_floats": c_int64, "uem_pcl_workspace_floats": c_int64,
-            "uem_loss_workspace_floats": c_int64}
+            "uem_loss_workspace_floats": c_int64, "uem_layernorm_workspace_floats": c_int64}
 
 # compile-time constants mirrored from the header
 UEM_MAX_CLASSES = 16
@@ -161,6 +164,7 @@ UEM_PROTO_SPLIT = 256
 UEM_NORM_BLOCKS = 1024
 CONV_IN_AFFINE, CONV_IN_RELU, CONV_ACCUMULATE, CONV_TRANSPOSED = 1, 2, 4, 8
 CONV_PREC_BF16 = 32
+LN_BF16, LN_PARAM_BF16 = 1, 2
 PREP_TRANSPOSE, PREP_WINO2, PREP_WINO2_T, PREP_WINO4, PREP_WINO4_T, PREP_STEM_PACK, PREP_TRANSPOSE_BF16 = range(7)
 
 

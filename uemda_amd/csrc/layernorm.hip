@@ -1,0 +1,443 @@
+// Layer normalisation over the last (channel) dimension of feature rows, forward and backward.
+//   y = (x - mean) * rstd * gamma + beta,   mean = sum x / C,   rstd = 1 / sqrt(sum (x - mean)^2 / C + eps)
+//   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),  g = dy * gamma,  xhat = (x - mean) * rstd
+//   dgamma = sum_rows dy * xhat,   dbeta = sum_rows dy
+// Bound by HBM: 2 row reads/writes forward, 3 backward, ~8 / ~14 flops an element.  A row is read ONCE: a team of lanes keeps it in
+// registers between the two sums of the statistics (the squares are summed about the mean, in 32 bits) and the output, so a row costs
+// its bytes and two reductions by lane exchange.  Backward, a team walks rows with its columns fixed, so dgamma / dbeta accumulate in
+// registers too; a block's teams are joined in LDS and the blocks' partial sums by a second small launch, in a fixed order: the result
+// does not depend on timing.
+#include "common.h"
+
+typedef unsigned short bf16_t;
+
+namespace {
+
+template <typename T> struct Vec;
+template <> struct Vec<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void load(const float* p, float* v) {
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+    }
+    static __device__ __forceinline__ void store(float* p, const float* v) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+    static __device__ __forceinline__ float load1(const float* p) { return *p; }
+    static __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+};
+template <> struct Vec<bf16_t> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ unsigned bits(float f) { return (unsigned)__builtin_bit_cast(unsigned short, (__bf16)f); }   // to nearest even: outputs are rounded once
+    static __device__ __forceinline__ void load(const bf16_t* p, float* v) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ void store(bf16_t* p, const float* v) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(bits(v[0]) | (bits(v[1]) << 16), bits(v[2]) | (bits(v[3]) << 16),
+                                                  bits(v[4]) | (bits(v[5]) << 16), bits(v[6]) | (bits(v[7]) << 16));
+    }
+    static __device__ __forceinline__ float load1(const bf16_t* p) { return __uint_as_float((uint32_t)*p << 16); }
+    static __device__ __forceinline__ void store1(bf16_t* p, float v) { *p = (bf16_t)bits(v); }
+};
+
+// gamma / beta are kept in 32 bits or bf16 independently of x
+__device__ __forceinline__ float param(const void* p, bool is16, int i) {
+    return is16 ? __uint_as_float((uint32_t)((const bf16_t*)p)[i] << 16) : ((const float*)p)[i];
+}
+
+struct LnP {
+    const void* x; const void* dy; const void* gamma; const void* beta;
+    void* y;                      // forward: y; backward: dx
+    float* mean; float* rstd;     // [rows] each; forward may be null (nothing to save)
+    float* part;                  // backward: [blocks][2][C] or null (no parameter gradients)
+    int64_t rows, x_ld, dy_ld;
+    int C, period;
+    float eps;
+    bool p16;
+};
+
+// How a row's elements fall to the accesses of its LPR lanes: access q = i * LPR + lane covers the columns q*W - shift ... + W - 1.
+//   MODE 0: rows start on 16-byte boundaries, 16-byte accesses, shift 0
+//   MODE 1: dense rows of any length: 16-byte accesses on the allocation's own boundaries, shift = the row's start modulo W; the row's
+//           first and last access go element by element.  Rows r and r + period start alike: a team walks rows of ONE start (r mod
+//           period), so that its columns stay fixed
+//   MODE 2: element by element (short rows that are not aligned)
+template <typename T, int LPR, int NV, int MODE>
+struct Row {
+    static constexpr int W = MODE == 2 ? 1 : Vec<T>::N;
+    static __device__ __forceinline__ int col(int i, int lane, int shift) { return (i * LPR + lane) * W - (MODE == 1 ? shift : 0); }
+    static __device__ __forceinline__ bool whole(int c, int C) { return MODE == 1 ? (c >= 0 && c + W <= C) : c < C; }
+    static __device__ __forceinline__ bool inside(int c, int C) { return MODE == 1 ? (c >= 0 && c < C) : true; }   // element of a !whole MODE 1 access
+    static __device__ __forceinline__ void load(const T* p, int C, int lane, int shift, bool on, float (*v)[W]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = col(i, lane, shift);
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[i][e] = 0.f;
+            if (on && whole(c, C)) {
+                if (MODE == 2) v[i][0] = Vec<T>::load1(p + c);
+                else Vec<T>::load(p + c, v[i]);
+            } else if (MODE == 1 && on) {
+#pragma unroll
+                for (int e = 0; e < W; ++e) if (inside(c + e, C)) v[i][e] = Vec<T>::load1(p + c + e);
+            }
+        }
+    }
+    static __device__ __forceinline__ void store(T* p, int C, int lane, int shift, const float (*v)[W]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = col(i, lane, shift);
+            if (whole(c, C)) {
+                if (MODE == 2) Vec<T>::store1(p + c, v[i][0]);
+                else Vec<T>::store(p + c, v[i]);
+            } else if (MODE == 1) {
+#pragma unroll
+                for (int e = 0; e < W; ++e) if (inside(c + e, C)) Vec<T>::store1(p + c + e, v[i][e]);
+            }
+        }
+    }
+    static __device__ __forceinline__ void params(const void* p, bool p16, float other, int C, int lane, int shift, float (*v)[W]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                const int c = col(i, lane, shift) + e;
+                v[i][e] = p != nullptr && c >= 0 && c < C ? param(p, p16, c) : other;
+            }
+    }
+};
+
+// sum over the LPR lanes of a team, in every lane of it; every lane of the block calls it (LPR = 256: `red` alternates between two
+// sets of four words, so one barrier a reduction is enough)
+template <int LPR>
+__device__ __forceinline__ float team_sum(float v, float* red, int& flip) {
+    if (LPR >= 64) v = wave_sum_dpp(v);
+    else {
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    }
+    if (LPR > 64) {
+        float* const r = red + flip * 4;
+        flip ^= 1;
+        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+        __syncthreads();
+        v = (r[0] + r[1]) + (r[2] + r[3]);
+    }
+    return v;
+}
+
+template <typename T, int LPR, int NV, int MODE>
+__global__ __launch_bounds__(256) void layernorm_fwd_kernel(const LnP p) {
+    using R = Row<T, LPR, NV, MODE>;
+    constexpr int W = R::W, TEAMS = 256 / LPR;
+    __shared__ float red[8];
+    int flip = 0;
+    const int lane = threadIdx.x % LPR;
+    const int64_t team = (int64_t)blockIdx.x * TEAMS + threadIdx.x / LPR, teams = (int64_t)gridDim.x * TEAMS;
+    const int shift = MODE == 1 ? (int)(((team % p.period) * p.C) & (W - 1)) : 0;      // teams % period == 0: all its rows start alike
+    const float inv = 1.f / (float)p.C;
+    float ga[NV][W], be[NV][W];
+    R::params(p.gamma, p.p16, 1.f, p.C, lane, shift, ga);
+    R::params(p.beta, p.p16, 0.f, p.C, lane, shift, be);
+    // the loop's bound is uniform over the block: every lane joins every exchange
+    for (int64_t base = (int64_t)blockIdx.x * TEAMS, r = team; base < p.rows; base += teams, r += teams) {
+        const bool on = r < p.rows;
+        float v[NV][W];
+        R::load((const T*)p.x + r * p.x_ld, p.C, lane, shift, on, v);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) s += v[i][e];
+        const float mean = team_sum<LPR>(s, red, flip) * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = R::col(i, lane, shift);
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                v[i][e] -= mean;
+                if (R::whole(c, p.C) || (MODE == 1 && R::inside(c + e, p.C))) q = fmaf(v[i][e], v[i][e], q);
+            }
+        }
+        const float rstd = 1.f / sqrtf(team_sum<LPR>(q, red, flip) * inv + p.eps);
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[i][e] = fmaf(v[i][e] * rstd, ga[i][e], be[i][e]);
+            R::store((T*)p.y + r * p.C, p.C, lane, shift, v);
+            if (p.mean != nullptr && lane == 0) { p.mean[r] = mean; p.rstd[r] = rstd; }
+        }
+    }
+}
+
+template <typename T, int LPR, int NV, int MODE>
+__global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
+    using R = Row<T, LPR, NV, MODE>;
+    constexpr int W = R::W, TEAMS = 256 / LPR, CAP = LPR > 64 ? 1 : LPR * NV * W;
+    __shared__ float red[8];
+    __shared__ float join[2][CAP];
+    int flip = 0;
+    const int lane = threadIdx.x % LPR;
+    const int64_t team = (int64_t)blockIdx.x * TEAMS + threadIdx.x / LPR, teams = (int64_t)gridDim.x * TEAMS;
+    const int shift = MODE == 1 ? (int)(((team % p.period) * p.C) & (W - 1)) : 0;
+    const float inv = 1.f / (float)p.C;
+    float ga[NV][W], aw[NV][W], ab[NV][W];
+    R::params(p.gamma, p.p16, 1.f, p.C, lane, shift, ga);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < W; ++e) aw[i][e] = ab[i][e] = 0.f;
+    for (int64_t base = (int64_t)blockIdx.x * TEAMS, r = team; base < p.rows; base += teams, r += teams) {
+        const bool on = r < p.rows;
+        float v[NV][W], g[NV][W];
+        R::load((const T*)p.x + r * p.x_ld, p.C, lane, shift, on, v);
+        R::load((const T*)p.dy + r * p.dy_ld, p.C, lane, shift, on, g);
+        const float mean = on ? p.mean[r] : 0.f, rstd = on ? p.rstd[r] : 0.f;
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                v[i][e] = (v[i][e] - mean) * rstd;                             // columns outside the row carry g = 0
+                aw[i][e] = fmaf(g[i][e], v[i][e], aw[i][e]);
+                ab[i][e] += g[i][e];
+                g[i][e] *= ga[i][e];
+                s1 += g[i][e];
+                s2 = fmaf(g[i][e], v[i][e], s2);
+            }
+        s1 = team_sum<LPR>(s1, red, flip) * inv;
+        s2 = team_sum<LPR>(s2, red, flip) * inv;
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[i][e] = rstd * (g[i][e] - s1 - v[i][e] * s2);
+            R::store((T*)p.y + r * p.C, p.C, lane, shift, v);
+        }
+    }
+    if (p.part == nullptr) return;
+    float* const out = p.part + (int64_t)blockIdx.x * 2 * p.C;
+    if (LPR > 64) {                                                            // one team a block: straight out
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) {
+                const int c = R::col(i, lane, shift) + e;
+                if (c >= 0 && c < p.C) { out[c] = aw[i][e]; out[p.C + c] = ab[i][e]; }
+            }
+        return;
+    }
+#pragma unroll
+    for (int o = LPR; o < 64; o <<= 1)                                         // the teams of a wave
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < W; ++e) { aw[i][e] += __shfl_xor(aw[i][e], o, 64); ab[i][e] += __shfl_xor(ab[i][e], o, 64); }
+    for (int w = 0; w < 4; ++w) {                                              // the waves, in order
+        if ((int)(threadIdx.x >> 6) == w && (threadIdx.x & 63) < LPR) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e) {
+                    const int c = R::col(i, lane, shift) + e;
+                    if (c >= 0 && c < p.C) {
+                        join[0][c] = aw[i][e] + (w ? join[0][c] : 0.f);
+                        join[1][c] = ab[i][e] + (w ? join[1][c] : 0.f);
+                    }
+                }
+        }
+        __syncthreads();
+    }
+    for (int c = threadIdx.x; c < p.C; c += 256) { out[c] = join[0][c]; out[p.C + c] = join[1][c]; }
+}
+
+// Any row length, any alignment: a block per row that reads the row again for each sum (rows beyond the register kernels' 8192
+// columns, or rows whose strides and bases share no 16-byte grid).  The parameter gradients are a separate pass over columns.
+template <typename T>
+__device__ __forceinline__ float block_sum(float v, float* red) {
+    v = wave_sum_dpp(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm_fwd_any_kernel(const LnP p) {
+    __shared__ float red[4];
+    const float inv = 1.f / (float)p.C;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const T* const x = (const T*)p.x + r * p.x_ld;
+        T* const y = (T*)p.y + r * p.C;
+        float s = 0.f, q = 0.f;
+        for (int c = threadIdx.x; c < p.C; c += 256) s += Vec<T>::load1(x + c);
+        const float mean = block_sum<T>(s, red) * inv;
+        for (int c = threadIdx.x; c < p.C; c += 256) { const float d = Vec<T>::load1(x + c) - mean; q = fmaf(d, d, q); }
+        const float rstd = 1.f / sqrtf(block_sum<T>(q, red) * inv + p.eps);
+        for (int c = threadIdx.x; c < p.C; c += 256) {
+            const float ga = p.gamma ? param(p.gamma, p.p16, c) : 1.f, be = p.beta ? param(p.beta, p.p16, c) : 0.f;
+            Vec<T>::store1(y + c, fmaf((Vec<T>::load1(x + c) - mean) * rstd, ga, be));
+        }
+        if (p.mean != nullptr && threadIdx.x == 0) { p.mean[r] = mean; p.rstd[r] = rstd; }
+    }
+}
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm_bwd_any_kernel(const LnP p) {
+    __shared__ float red[4];
+    const float inv = 1.f / (float)p.C;
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const T* const x = (const T*)p.x + r * p.x_ld;
+        const T* const dy = (const T*)p.dy + r * p.dy_ld;
+        T* const dx = (T*)p.y + r * p.C;
+        const float mean = p.mean[r], rstd = p.rstd[r];
+        float s1 = 0.f, s2 = 0.f;
+        for (int c = threadIdx.x; c < p.C; c += 256) {
+            const float g = Vec<T>::load1(dy + c) * (p.gamma ? param(p.gamma, p.p16, c) : 1.f);
+            s1 += g;
+            s2 = fmaf(g, (Vec<T>::load1(x + c) - mean) * rstd, s2);
+        }
+        s1 = block_sum<T>(s1, red) * inv;
+        s2 = block_sum<T>(s2, red) * inv;
+        for (int c = threadIdx.x; c < p.C; c += 256) {
+            const float g = Vec<T>::load1(dy + c) * (p.gamma ? param(p.gamma, p.p16, c) : 1.f);
+            Vec<T>::store1(dx + c, rstd * (g - s1 - (Vec<T>::load1(x + c) - mean) * rstd * s2));
+        }
+    }
+}
+// 64 columns x 4 row lanes a block, rows shared out over gridDim.y
+template <typename T>
+__global__ __launch_bounds__(256) void layernorm_cols_kernel(const LnP p) {
+    __shared__ float join[2][4][64];
+    const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    float a = 0.f, b = 0.f;
+    if (c < p.C)
+        for (int64_t r = (int64_t)blockIdx.y * 4 + w; r < p.rows; r += (int64_t)gridDim.y * 4) {
+            const float g = Vec<T>::load1((const T*)p.dy + r * p.dy_ld + c);
+            a = fmaf(g, (Vec<T>::load1((const T*)p.x + r * p.x_ld + c) - p.mean[r]) * p.rstd[r], a);
+            b += g;
+        }
+    join[0][w][threadIdx.x & 63] = a;
+    join[1][w][threadIdx.x & 63] = b;
+    __syncthreads();
+    if (w < 2 && c < p.C) {
+        const float* const j = &join[w][0][threadIdx.x & 63];
+        p.part[((int64_t)blockIdx.y * 2 + w) * p.C + c] = (j[0] + j[64]) + (j[128] + j[192]);
+    }
+}
+
+// dgamma / dbeta = the blocks' partial sums, added in block order: 16 columns x 16 slices of the blocks a block
+__global__ __launch_bounds__(256) void layernorm_params_kernel(const float* __restrict__ part, int nb, int C, void* dgamma, void* dbeta, bool p16) {
+    __shared__ float join[16][17];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), sl = threadIdx.x >> 4;
+    float s = 0.f;
+    if (col < 2 * C)
+        for (int b = sl; b < nb; b += 16) s += part[(int64_t)b * 2 * C + col];
+    join[sl][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (sl == 0 && col < 2 * C) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += join[i][threadIdx.x];
+        void* const out = col < C ? dgamma : dbeta;
+        const int c = col < C ? col : col - C;
+        if (out != nullptr) {
+            if (p16) Vec<bf16_t>::store1((bf16_t*)out + c, t);
+            else ((float*)out)[c] = t;
+        }
+    }
+}
+
+constexpr int LN_BWD_BLOCKS = 1024;            // most partial sums the backward leaves
+
+template <typename T, int LPR, int NV, int MODE>
+int go(const LnP& p, bool bwd, hipStream_t st) {
+    constexpr int TEAMS = 256 / LPR;
+    int64_t nb = uem_cdiv(p.rows, TEAMS);
+    const int64_t most = bwd ? LN_BWD_BLOCKS : 256 * 16;
+    if (nb > most) nb = most;
+    if (MODE == 1) nb = uem_cdiv(nb, 8) * 8;                                   // teams % period == 0 (period <= 8)
+    if (bwd) layernorm_bwd_kernel<T, LPR, NV, MODE><<<(int)nb, 256, 0, st>>>(p);
+    else layernorm_fwd_kernel<T, LPR, NV, MODE><<<(int)nb, 256, 0, st>>>(p);
+    return (int)nb;
+}
+
+template <typename T>
+int run(LnP p, bool bwd, hipStream_t st) {
+    constexpr int W = Vec<T>::N;
+    const uintptr_t bases = (uintptr_t)p.x | (uintptr_t)p.y | (bwd ? (uintptr_t)p.dy : 0);
+    const bool base16 = (bases & 15) == 0;
+    const bool dense = p.x_ld == p.C && (!bwd || p.dy_ld == p.C);
+    p.period = 1;
+    // Lanes per row: one wave while a lane holds at most 16 elements (8 in bf16's wide accesses), a block of four above -- backward keeps
+    // five values an element in registers (x, g, gamma and the two parameter gradients), 32 elements a lane would leave two waves a SIMD
+    if (base16 && p.C % W == 0 && p.x_ld % W == 0 && (!bwd || p.dy_ld % W == 0)) {
+        const int v = p.C / W;
+        if (v <= 8) return go<T, 8, 1, 0>(p, bwd, st);
+        if (v <= 16) return go<T, 16, 1, 0>(p, bwd, st);
+        if (v <= 32) return go<T, 32, 1, 0>(p, bwd, st);
+        if (v <= 64) return go<T, 64, 1, 0>(p, bwd, st);
+        if (v <= 128) return go<T, 64, 2, 0>(p, bwd, st);
+        if (v <= 256) return go<T, 256, 1, 0>(p, bwd, st);
+        if (v <= 512) return go<T, 256, 2, 0>(p, bwd, st);
+        if (v <= 1024) return go<T, 256, 4, 0>(p, bwd, st);
+        if (W == 4 && v <= 2048) return go<T, 256, W == 4 ? 8 : 4, 0>(p, bwd, st);
+    } else if (p.C <= 256) {
+        if (p.C <= 8) return go<T, 8, 1, 2>(p, bwd, st);
+        if (p.C <= 32) return go<T, 32, 1, 2>(p, bwd, st);
+        if (p.C <= 64) return go<T, 64, 1, 2>(p, bwd, st);
+        return go<T, 64, 4, 2>(p, bwd, st);
+    } else if (base16 && dense) {
+        const int v = (p.C + W - 1 + W - 1) / W;                               // accesses of the worst start
+        p.period = W;
+        while (p.period > 1 && ((int64_t)(p.period / 2) * p.C) % W == 0) p.period /= 2;
+        if (v <= 128) return go<T, 64, 2, 1>(p, bwd, st);
+        if (v <= 256) return go<T, 256, 1, 1>(p, bwd, st);
+        if (v <= 512) return go<T, 256, 2, 1>(p, bwd, st);
+        if (v <= 1024) return go<T, 256, 4, 1>(p, bwd, st);
+        if (W == 4 && v <= 2048) return go<T, 256, W == 4 ? 8 : 4, 1>(p, bwd, st);
+    }
+    const int nb = p.rows < 256 * 16 ? (int)p.rows : 256 * 16;
+    if (!bwd) { layernorm_fwd_any_kernel<T><<<nb, 256, 0, st>>>(p); return nb; }
+    layernorm_bwd_any_kernel<T><<<nb, 256, 0, st>>>(p);
+    if (p.part == nullptr) return nb;
+    const int ny = (int)(uem_cdiv(p.rows, 4) < 64 ? uem_cdiv(p.rows, 4) : 64);
+    layernorm_cols_kernel<T><<<dim3((unsigned)uem_cdiv(p.C, 64), (unsigned)ny), 256, 0, st>>>(p);
+    return ny;
+}
+
+}  // namespace
+
+extern "C" int64_t uem_layernorm_workspace_floats(int64_t rows, int C) {
+    int64_t nb = rows < LN_BWD_BLOCKS ? uem_cdiv(rows, 8) * 8 : LN_BWD_BLOCKS;
+    return nb * 2 * (int64_t)C;
+}
+extern "C" int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
+                                 int64_t rows, int C, float eps, int flags, void* stream) {
+    UEM_REQUIRE(x && y && rows > 0 && C > 0 && x_ld >= C, "layernorm_fwd: bad arguments (rows, C > 0, x_ld >= C)");
+    UEM_REQUIRE((mean == nullptr) == (rstd == nullptr), "layernorm_fwd: mean and rstd go together");
+    UEM_REQUIRE((flags & ~(UEM_LN_BF16 | UEM_LN_PARAM_BF16)) == 0, "layernorm_fwd: unknown flags %d", flags);
+    LnP p{};
+    p.x = x; p.gamma = gamma; p.beta = beta; p.y = y; p.mean = mean; p.rstd = rstd; p.rows = rows; p.x_ld = x_ld; p.C = C; p.eps = eps;
+    p.p16 = (flags & UEM_LN_PARAM_BF16) != 0;
+    if (flags & UEM_LN_BF16) run<bf16_t>(p, false, (hipStream_t)stream);
+    else run<float>(p, false, (hipStream_t)stream);
+    return uem_check_launch("layernorm_fwd");
+}
+extern "C" int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const void* gamma, const float* mean,
+                                 const float* rstd, void* dx, void* dgamma, void* dbeta, float* workspace, int64_t rows, int C, int flags,
+                                 void* stream) {
+    UEM_REQUIRE(x && dy && mean && rstd && dx && rows > 0 && C > 0 && x_ld >= C && dy_ld >= C,
+                "layernorm_bwd: bad arguments (rows, C > 0, strides >= C)");
+    UEM_REQUIRE((dgamma == nullptr && dbeta == nullptr) || workspace, "layernorm_bwd: parameter gradients need the workspace");
+    UEM_REQUIRE((flags & ~(UEM_LN_BF16 | UEM_LN_PARAM_BF16)) == 0, "layernorm_bwd: unknown flags %d", flags);
+    LnP p{};
+    p.x = x; p.dy = dy; p.gamma = gamma; p.y = dx; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
+    p.part = dgamma || dbeta ? workspace : nullptr;
+    p.rows = rows; p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = C; p.p16 = (flags & UEM_LN_PARAM_BF16) != 0;
+    hipStream_t st = (hipStream_t)stream;
+    const int nb = (flags & UEM_LN_BF16) ? run<bf16_t>(p, true, st) : run<float>(p, true, st);
+    if (p.part) layernorm_params_kernel<<<(int)uem_cdiv(2 * (int64_t)C, 16), 256, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
+    return uem_check_launch("layernorm_bwd");
+}
