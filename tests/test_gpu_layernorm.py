@@ -186,6 +186,15 @@ def test_gradient_against_differences():
         assert abs(got - exact) <= rounding + 1.5 * curve + 1e-6, (name, float(got), float(exact), float(rounding), float(curve))
 
 
+def test_a_second_derivative_is_refused():
+    from uemda_amd import UemError
+    from uemda_amd.norm import layer_norm
+    x = torch.randn(4, 8, device="cuda", requires_grad=True)
+    y = layer_norm(x)
+    with pytest.raises(UemError, match="gradient of the gradient"):
+        torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_results_repeat_and_a_captured_step_replays():
     from uemda_amd.norm import layer_norm
     x, w, b, dy = data(4097, 320, torch.bfloat16, 17)

@@ -69,18 +69,27 @@ struct Row {
     static __device__ __forceinline__ int col(int i, int lane, int shift) { return (i * LPR + lane) * W - (MODE == 1 ? shift : 0); }
     static __device__ __forceinline__ bool whole(int c, int C) { return MODE == 1 ? (c >= 0 && c + W <= C) : c < C; }
     static __device__ __forceinline__ bool inside(int c, int C) { return MODE == 1 ? (c >= 0 && c < C) : true; }   // element of a !whole MODE 1 access
-    static __device__ __forceinline__ void load(const T* p, int C, int lane, int shift, bool on, float (*v)[W]) {
+    // `end`: no access may reach past this element of the row (the allocation's last one, seen from the row).  A row's outer accesses
+    // hold elements of the neighbouring rows: read whole and masked, so that every lane's row is one load an access; only the very last
+    // row of the tensor has to pick its tail's elements one by one
+    static __device__ __forceinline__ void load(const T* p, int C, int lane, int shift, bool on, int64_t end, float (*v)[W]) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = col(i, lane, shift);
 #pragma unroll
             for (int e = 0; e < W; ++e) v[i][e] = 0.f;
-            if (on && whole(c, C)) {
+            if (MODE == 1) {
+                if (on && c < C) {
+                    if (c + W <= end) Vec<T>::load(p + c, v[i]);
+                    else
+#pragma unroll
+                        for (int e = 0; e < W; ++e) if (inside(c + e, C)) v[i][e] = Vec<T>::load1(p + c + e);
+                }
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[i][e] = inside(c + e, C) ? v[i][e] : 0.f;
+            } else if (on && c < C) {
                 if (MODE == 2) v[i][0] = Vec<T>::load1(p + c);
                 else Vec<T>::load(p + c, v[i]);
-            } else if (MODE == 1 && on) {
-#pragma unroll
-                for (int e = 0; e < W; ++e) if (inside(c + e, C)) v[i][e] = Vec<T>::load1(p + c + e);
             }
         }
     }
@@ -99,32 +108,52 @@ struct Row {
     }
     static __device__ __forceinline__ void params(const void* p, bool p16, float other, int C, int lane, int shift, float (*v)[W]) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            const int c0 = col(i, lane, shift);
+            if (MODE != 2 && p != nullptr && !p16 && whole(c0, C)) {           // fp32: 16 bytes at a time, on any 4-byte boundary
+#pragma unroll
+                for (int e = 0; e < W; e += 4) {
+                    struct __attribute__((packed, aligned(4))) F4 { float f[4]; };
+                    const F4 u = *reinterpret_cast<const F4*>((const float*)p + c0 + e);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[i][e + k] = u.f[k];
+                }
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < W; ++e) {
-                const int c = col(i, lane, shift) + e;
+                const int c = c0 + e;
                 v[i][e] = p != nullptr && c >= 0 && c < C ? param(p, p16, c) : other;
             }
+        }
     }
 };
 
-// sum over the LPR lanes of a team, in every lane of it; every lane of the block calls it (LPR = 256: `red` alternates between two
-// sets of four words, so one barrier a reduction is enough)
-template <int LPR>
-__device__ __forceinline__ float team_sum(float v, float* red, int& flip) {
-    if (LPR >= 64) v = wave_sum_dpp(v);
-    else {
+// Sums of K values over the LPR lanes of a team, in every lane of it; every lane of the block calls it.  Inside a row of 16 lanes by DPP
+// (no LDS round trips: exchange with lane ^ 1, ^ 2, then the mirrored half and the mirrored row); a block's four waves through `red`,
+// which alternates between two sets of words, so that one barrier a reduction is enough.
+template <int LPR, int K>
+__device__ __forceinline__ void team_sums(float (&v)[K], float* red, int& flip) {
 #pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    for (int k = 0; k < K; ++k) {
+        if (LPR >= 64) { v[k] = wave_sum_dpp(v[k]); continue; }
+        v[k] += dpp_take0<0xB1, 0xF>(v[k]);
+        v[k] += dpp_take0<0x4E, 0xF>(v[k]);
+        v[k] += dpp_take0<0x141, 0xF>(v[k]);
+        if (LPR >= 16) v[k] += dpp_take0<0x140, 0xF>(v[k]);
+        if (LPR >= 32) v[k] += __shfl_xor(v[k], 16, 64);
     }
     if (LPR > 64) {
-        float* const r = red + flip * 4;
+        float* const r = red + flip * 4 * K;
         flip ^= 1;
-        if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) r[(threadIdx.x >> 6) * K + k] = v[k];
+        }
         __syncthreads();
-        v = (r[0] + r[1]) + (r[2] + r[3]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) v[k] = (r[k] + r[K + k]) + (r[2 * K + k] + r[3 * K + k]);
     }
-    return v;
 }
 
 template <typename T, int LPR, int NV, int MODE>
@@ -143,41 +172,43 @@ __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const LnP p) {
     // the loop's bound is uniform over the block: every lane joins every exchange
     for (int64_t base = (int64_t)blockIdx.x * TEAMS, r = team; base < p.rows; base += teams, r += teams) {
         const bool on = r < p.rows;
-        float v[NV][W];
-        R::load((const T*)p.x + r * p.x_ld, p.C, lane, shift, on, v);
-        float s = 0.f;
+        float v[NV][W], s[1] = {0.f};
+        R::load((const T*)p.x + r * p.x_ld, p.C, lane, shift, on, (p.rows - r) * p.x_ld, v);
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int e = 0; e < W; ++e) s += v[i][e];
-        const float mean = team_sum<LPR>(s, red, flip) * inv;
-        float q = 0.f;
+            for (int e = 0; e < W; ++e) s[0] += v[i][e];
+        team_sums<LPR, 1>(s, red, flip);
+        const float mean = s[0] * inv;
+        s[0] = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = R::col(i, lane, shift);
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 v[i][e] -= mean;
-                if (R::whole(c, p.C) || (MODE == 1 && R::inside(c + e, p.C))) q = fmaf(v[i][e], v[i][e], q);
+                const bool in = MODE == 1 ? R::inside(c + e, p.C) : c < p.C;
+                s[0] = in ? fmaf(v[i][e], v[i][e], s[0]) : s[0];
             }
         }
-        const float rstd = 1.f / sqrtf(team_sum<LPR>(q, red, flip) * inv + p.eps);
-        if (on) {
+        team_sums<LPR, 1>(s, red, flip);
+        const float rstd = 1.f / sqrtf(s[0] * inv + p.eps);
+        if (!on) continue;
 #pragma unroll
-            for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < W; ++e) v[i][e] = fmaf(v[i][e] * rstd, ga[i][e], be[i][e]);
-            R::store((T*)p.y + r * p.C, p.C, lane, shift, v);
-            if (p.mean != nullptr && lane == 0) { p.mean[r] = mean; p.rstd[r] = rstd; }
-        }
+            for (int e = 0; e < W; ++e) v[i][e] = fmaf(v[i][e] * rstd, ga[i][e], be[i][e]);
+        R::store((T*)p.y + r * p.C, p.C, lane, shift, v);
+        if (p.mean != nullptr && lane == 0) { p.mean[r] = mean; p.rstd[r] = rstd; }
     }
 }
 
-template <typename T, int LPR, int NV, int MODE>
+// U rows of a team are in flight together: their loads are issued before the first reduction
+template <typename T, int LPR, int NV, int MODE, int U>
 __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
     using R = Row<T, LPR, NV, MODE>;
     constexpr int W = R::W, TEAMS = 256 / LPR, CAP = LPR > 64 ? 1 : LPR * NV * W;
-    __shared__ float red[8];
+    __shared__ float red[16 * U];
     __shared__ float join[2][CAP];
     int flip = 0;
     const int lane = threadIdx.x % LPR;
@@ -190,32 +221,46 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < W; ++e) aw[i][e] = ab[i][e] = 0.f;
-    for (int64_t base = (int64_t)blockIdx.x * TEAMS, r = team; base < p.rows; base += teams, r += teams) {
-        const bool on = r < p.rows;
-        float v[NV][W], g[NV][W];
-        R::load((const T*)p.x + r * p.x_ld, p.C, lane, shift, on, v);
-        R::load((const T*)p.dy + r * p.dy_ld, p.C, lane, shift, on, g);
-        const float mean = on ? p.mean[r] : 0.f, rstd = on ? p.rstd[r] : 0.f;
-        float s1 = 0.f, s2 = 0.f;
+    for (int64_t base = (int64_t)blockIdx.x * TEAMS, r = team; base < p.rows; base += teams * U, r += teams * U) {
+        float v[U][NV][W], g[U][NV][W], mean[U], rstd[U], s[2 * U];
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int u = 0; u < U; ++u) {
+            const int64_t ru = r + u * teams;
+            const bool on = ru < p.rows;
+            R::load((const T*)p.x + ru * p.x_ld, p.C, lane, shift, on, (p.rows - ru) * p.x_ld, v[u]);
+            R::load((const T*)p.dy + ru * p.dy_ld, p.C, lane, shift, on, (p.rows - ru) * p.dy_ld, g[u]);
+            mean[u] = on ? p.mean[ru] : 0.f;
+            rstd[u] = on ? p.rstd[ru] : 0.f;
+        }
 #pragma unroll
-            for (int e = 0; e < W; ++e) {
-                v[i][e] = (v[i][e] - mean) * rstd;                             // columns outside the row carry g = 0
-                aw[i][e] = fmaf(g[i][e], v[i][e], aw[i][e]);
-                ab[i][e] += g[i][e];
-                g[i][e] *= ga[i][e];
-                s1 += g[i][e];
-                s2 = fmaf(g[i][e], v[i][e], s2);
-            }
-        s1 = team_sum<LPR>(s1, red, flip) * inv;
-        s2 = team_sum<LPR>(s2, red, flip) * inv;
-        if (on) {
+        for (int u = 0; u < U; ++u) {
+            float s1 = 0.f, s2 = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < W; ++e) v[i][e] = rstd * (g[i][e] - s1 - v[i][e] * s2);
-            R::store((T*)p.y + r * p.C, p.C, lane, shift, v);
+                for (int e = 0; e < W; ++e) {
+                    const float h = (v[u][i][e] - mean[u]) * rstd[u];          // columns outside the row carry dy = 0
+                    v[u][i][e] = h;
+                    aw[i][e] = fmaf(g[u][i][e], h, aw[i][e]);
+                    ab[i][e] += g[u][i][e];
+                    g[u][i][e] *= ga[i][e];
+                    s1 += g[u][i][e];
+                    s2 = fmaf(g[u][i][e], h, s2);
+                }
+            s[2 * u] = s1;
+            s[2 * u + 1] = s2;
+        }
+        team_sums<LPR, 2 * U>(s, red, flip);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t ru = r + u * teams;
+            if (ru >= p.rows) continue;
+            const float s1 = s[2 * u] * inv, s2 = s[2 * u + 1] * inv;
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < W; ++e) v[u][i][e] = rstd[u] * (g[u][i][e] - s1 - v[u][i][e] * s2);
+            R::store((T*)p.y + ru * p.C, p.C, lane, shift, v[u]);
         }
     }
     if (p.part == nullptr) return;
@@ -327,24 +372,29 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(const LnP p) {
     }
 }
 
-// dgamma / dbeta = the blocks' partial sums, added in block order: 16 columns x 16 slices of the blocks a block
-__global__ __launch_bounds__(256) void layernorm_params_kernel(const float* __restrict__ part, int nb, int C, void* dgamma, void* dbeta, bool p16) {
-    __shared__ float join[16][17];
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), sl = threadIdx.x >> 4;
+// dgamma / dbeta = the blocks' partial sums, added in a fixed order: 16 columns x 64 slices of the blocks a block of 1024 threads
+__global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __restrict__ part, int nb, int C, void* dgamma, void* dbeta, bool p16) {
+    __shared__ float join[64][17];
+    const int t = threadIdx.x & 15, sl = threadIdx.x >> 4;
+    const int64_t col = (int64_t)blockIdx.x * 16 + t, n = 2 * (int64_t)C;
     float s = 0.f;
-    if (col < 2 * C)
-        for (int b = sl; b < nb; b += 16) s += part[(int64_t)b * 2 * C + col];
-    join[sl][threadIdx.x & 15] = s;
+    if (col < n) {
+#pragma unroll 8
+        for (int b = sl; b < nb; b += 64) s += part[b * n + col];
+    }
+    join[sl][t] = s;
     __syncthreads();
-    if (sl == 0 && col < 2 * C) {
-        float t = 0.f;
+    if (sl < 4) {
+        float q = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += join[i][threadIdx.x];
+        for (int i = 0; i < 16; ++i) q += join[sl * 16 + i][t];
+        q += __shfl_xor(q, 16, 64);
+        q += __shfl_xor(q, 32, 64);
         void* const out = col < C ? dgamma : dbeta;
-        const int c = col < C ? col : col - C;
-        if (out != nullptr) {
-            if (p16) Vec<bf16_t>::store1((bf16_t*)out + c, t);
-            else ((float*)out)[c] = t;
+        const int64_t c = col < C ? col : col - C;
+        if (sl == 0 && col < n && out != nullptr) {
+            if (p16) Vec<bf16_t>::store1((bf16_t*)out + c, q);
+            else ((float*)out)[c] = q;
         }
     }
 }
@@ -353,12 +403,17 @@ constexpr int LN_BWD_BLOCKS = 1024;            // most partial sums the backward
 
 template <typename T, int LPR, int NV, int MODE>
 int go(const LnP& p, bool bwd, hipStream_t st) {
-    constexpr int TEAMS = 256 / LPR;
-    int64_t nb = uem_cdiv(p.rows, TEAMS);
-    const int64_t most = bwd ? LN_BWD_BLOCKS : 256 * 16;
+    // Measured, us (fp32 32768 x 2048 | bf16 524288 x 256 | bf16 65536 x 777; a plain copy of the map takes 100 | 101 | 29):
+    //   forward, grid of at most 1024 / 4096 / 16384 blocks: 97 / 99 / 91 | 103 / 108 / 100 | 42 / 42 / 69; two rows in flight a team gain
+    //   nothing (92 | 100 | 56).  So: no cap worth the name on the 16-byte grid, 1024 blocks where a team's parameters cost more to load.
+    //   backward, 512 / 1024 / 2048 blocks: one row 146 / 165 / 172 | 259 / 168 / 184 | 126 / 134 / 124, two rows 154 / 169 / 179 |
+    //   235 / 157 / 162 | 125 / 133 / 150: every block costs its partial sums; two rows only where a team is part of a wave.
+    constexpr int UB = LPR < 64 ? 2 : 1, TEAMS = 256 / LPR;
+    int64_t nb = uem_cdiv(p.rows, TEAMS * (bwd ? UB : 1));
+    const int64_t most = bwd ? (LPR > 64 || MODE == 1 ? LN_BWD_BLOCKS / 2 : LN_BWD_BLOCKS) : MODE == 0 ? 16384 : 1024;
     if (nb > most) nb = most;
     if (MODE == 1) nb = uem_cdiv(nb, 8) * 8;                                   // teams % period == 0 (period <= 8)
-    if (bwd) layernorm_bwd_kernel<T, LPR, NV, MODE><<<(int)nb, 256, 0, st>>>(p);
+    if (bwd) layernorm_bwd_kernel<T, LPR, NV, MODE, UB><<<(int)nb, 256, 0, st>>>(p);
     else layernorm_fwd_kernel<T, LPR, NV, MODE><<<(int)nb, 256, 0, st>>>(p);
     return (int)nb;
 }
@@ -438,6 +493,6 @@ extern "C" int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, in
     p.rows = rows; p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = C; p.p16 = (flags & UEM_LN_PARAM_BF16) != 0;
     hipStream_t st = (hipStream_t)stream;
     const int nb = (flags & UEM_LN_BF16) ? run<bf16_t>(p, true, st) : run<float>(p, true, st);
-    if (p.part) layernorm_params_kernel<<<(int)uem_cdiv(2 * (int64_t)C, 16), 256, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
+    if (p.part) layernorm_params_kernel<<<(int)uem_cdiv(2 * (int64_t)C, 16), 1024, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
     return uem_check_launch("layernorm_bwd");
 }

@@ -5,7 +5,6 @@ mean and variance.  x is fp32 or bf16, statistics and sums are fp32; weight and 
 import torch
 import torch.nn as nn
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 from .ops import UemError, call, ptr, stream
@@ -22,9 +21,12 @@ def _rows(t, c):
     return t.contiguous(), c
 
 
-def _flags(x, weight, bias):
-    p = weight if weight is not None else bias
-    return (_lib.LN_BF16 if x.dtype == torch.bfloat16 else 0) | (_lib.LN_PARAM_BF16 if p is not None and p.dtype == torch.bfloat16 else 0)
+def _flags(x, param_dtype):
+    return (_lib.LN_BF16 if x.dtype == torch.bfloat16 else 0) | (_lib.LN_PARAM_BF16 if param_dtype == torch.bfloat16 else 0)
+
+
+def _param_dtype(weight, bias):
+    return weight.dtype if weight is not None else bias.dtype if bias is not None else None
 
 
 def _forward(x, weight, bias, eps, save):
@@ -34,9 +36,10 @@ def _forward(x, weight, bias, eps, save):
     stats = torch.empty((2, rows), device=x.device, dtype=torch.float32) if save else None
     if rows:
         x, ld = _rows(x, c)
-        with torch.cuda.device(x.device):
-            call("uem_layernorm_fwd", ptr(x), ld, ptr(weight), ptr(bias), ptr(y), ptr(stats[0]) if save else None, ptr(stats[1]) if save else None,
-                 rows, c, eps, _flags(x, weight, bias), stream())
+        mean = ptr(stats)
+        with ops.on_device_of(x):
+            call("uem_layernorm_fwd", ptr(x), ld, ptr(weight), ptr(bias), ptr(y), mean, mean + 4 * rows if save else None, rows, c, eps,
+                 _flags(x, _param_dtype(weight, bias)), stream())
     return y, stats
 
 
@@ -45,32 +48,31 @@ class _LayerNormFn(Function):
     def forward(ctx, x, weight, bias, eps):
         y, stats = _forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.param_dtype = _param_dtype(weight, bias)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        ops.no_second_derivative("layer_norm")
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         c = x.shape[-1]
         rows = x.numel() // c
         dev = x.device
         dx = torch.empty(x.shape, device=dev, dtype=x.dtype)
-        dw = torch.empty(c, device=dev, dtype=weight.dtype) if need_w else None
-        db = torch.empty(c, device=dev, dtype=ctx.bias_dtype) if need_b else None
+        dw = torch.empty(c, device=dev, dtype=ctx.param_dtype) if need_w else None
+        db = torch.empty(c, device=dev, dtype=ctx.param_dtype) if need_b else None
         if rows == 0:
             return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None
         xr, x_ld = _rows(x, c)
         dyr, dy_ld = _rows(dy, c)
-        p = weight if weight is not None else db
-        flags = (_lib.LN_BF16 if x.dtype == torch.bfloat16 else 0) | (_lib.LN_PARAM_BF16 if p is not None and p.dtype == torch.bfloat16 else 0)
         ws = None
         if need_w or need_b:
             ws = torch.empty(_lib.load().uem_layernorm_workspace_floats(rows, c), device=dev, dtype=torch.float32)
-        with torch.cuda.device(dev):
-            call("uem_layernorm_bwd", ptr(xr), x_ld, ptr(dyr), dy_ld, ptr(weight), ptr(stats[0]), ptr(stats[1]), ptr(dx), ptr(dw), ptr(db), ptr(ws),
-                 rows, c, flags, stream())
+        mean = ptr(stats)
+        with ops.on_device_of(x):
+            call("uem_layernorm_bwd", ptr(xr), x_ld, ptr(dyr), dy_ld, ptr(weight), mean, mean + 4 * rows, ptr(dx), ptr(dw), ptr(db), ptr(ws),
+                 rows, c, _flags(x, ctx.param_dtype), stream())
         return dx if need_x else None, dw, db, None
 
 
