@@ -502,6 +502,19 @@ int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma, const void
 int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const void* gamma, const float* mean, const float* rstd,
                       void* dx, void* dgamma, void* dbeta, float* workspace, int64_t rows, int C, int flags, void* stream);
 
+/* ---- global norm over many tensors, and clipping ------------------------------------------------------------------------------
+ * ptrs / numels / bf16 are HOST arrays of `count` entries (read before the call returns): device address, elements, 1 = bf16 or 0 = fp32
+ * of each tensor; a tensor may begin at any element and may be empty.  norm_type 2: sqrt of the sum of squares (summed in 64 bits, in a
+ * fixed order); 0: largest magnitude.  norm_out: one device float.  partial: uem_multi_norm_workspace_doubles(count) device doubles.
+ * uem_multi_clip also scales every tensor in place by min(max_norm / (norm + 1e-6), 1) (torch.nn.utils.clip_grad_norm_) and writes nothing
+ * where that is 1; tensors that share memory are refused.                                                                          */
+#define UEM_MULTI_BLOCKS 8192
+int64_t uem_multi_norm_workspace_doubles(int count);   /* UEM_MULTI_BLOCKS + 2 * count */
+int uem_multi_norm(const uint64_t* ptrs, const int64_t* numels, const uint8_t* bf16, int count, int norm_type, double* partial,
+                   float* norm_out, void* stream);
+int uem_multi_clip(const uint64_t* ptrs, const int64_t* numels, const uint8_t* bf16, int count, int norm_type, double* partial,
+                   float* norm_out, float max_norm, void* stream);
+
 /* ---- data parallel (new relative to the reference, which is single-GPU: SURVEY 2a, 8e) --------------------------
  * all-reduce(sum, in place) of a flat fp32 buffer -- the gradient arena, 98 MB for R50-ASPP -- over RCCL on `stream`:
  * one process per GPU, xGMI inside the node.  Rank 0 draws an id with uem_comm_unique_id, the host ships those 128

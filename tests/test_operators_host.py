@@ -45,3 +45,37 @@ def test_layer_norm_formula_against_differences():
         t.copy_(t0 - h * v); down = (reference(x, w, b, dy, 1e-5)[0] * dy).sum()
         t.copy_(t0)
         assert abs((up - down) / (2 * h) - (grad * v).sum()) < 1e-7 * (1 + (grad * v).abs().sum())
+
+
+def test_gradient_norm_refusals():
+    from uemda_amd.optim import clip_grad_norm_, get_total_norm
+    p = torch.ones(3, requires_grad=True)
+    p.grad = torch.ones(3)
+    with pytest.raises(UemError, match="MI355X"):
+        get_total_norm([p.grad])
+    with pytest.raises(UemError, match="MI355X"):
+        clip_grad_norm_([p], 1.0)
+    with pytest.raises(UemError, match="norm_type"):
+        clip_grad_norm_([p], 1.0, norm_type=3)
+    with pytest.raises(UemError, match="negative"):
+        clip_grad_norm_([p], -1.0)
+    with pytest.raises(UemError, match="negative"):
+        clip_grad_norm_([p], float("nan"))
+    with pytest.raises(UemError, match="expected tensors"):
+        get_total_norm([1.0])
+    p.grad = torch.ones(3).to_sparse()
+    with pytest.raises(UemError, match="dense"):
+        clip_grad_norm_([p], 1.0)
+    assert float(get_total_norm([])) == 0.0 and float(clip_grad_norm_([], 1.0)) == 0.0
+    lib = _lib.load()
+    from array import array
+    ptrs, n = array("Q", [16, 20]), array("q", [2, 4])
+    args = (ptrs.buffer_info()[0], n.buffer_info()[0])
+    assert lib.uem_multi_clip(*args, b"\0\0", 2, 2, 16, 16, 1.0, None) == -1 and b"share memory" in lib.uem_last_error()
+    assert lib.uem_multi_norm(*args, b"\0\0", 2, 3, 16, 16, None) == -1 and b"norm type" in lib.uem_last_error()
+    assert lib.uem_multi_norm(*args, b"\0\0", -1, 2, 16, 16, None) == -1
+    ptrs[0] = 18
+    assert lib.uem_multi_norm(*args, b"\0\0", 2, 2, 16, 16, None) == -1 and b"element boundary" in lib.uem_last_error()
+    ptrs[0] = 0
+    assert lib.uem_multi_norm(*args, b"\0\0", 2, 2, 16, 16, None) == -1
+    assert lib.uem_multi_norm_workspace_doubles(3) == _lib.UEM_MULTI_BLOCKS + 6

@@ -147,6 +147,9 @@ SIGNATURES = {
     "uem_layernorm_workspace_floats": [L, I],
     "uem_layernorm_fwd": [P, L, P, P, P, P, P, L, I, F, I, P],
     "uem_layernorm_bwd": [P, L, P, L, P, P, P, P, P, P, P, L, I, I, P],
+    "uem_multi_norm_workspace_doubles": [I],
+    "uem_multi_norm": [P, P, P, I, I, P, P, P],
+    "uem_multi_clip": [P, P, P, I, I, P, P, F, P],
     "uem_comm_unique_id": [P],
     "uem_comm_init": [POINTER(c_void_p), P, I, I],
     "uem_allreduce_flat": [P, P, L, P],
@@ -156,12 +159,14 @@ SIGNATURES = {
 }
 _RESTYPE = {"uem_last_error": c_char_p, "uem_bn_workspace_floats": c_int64,
             "uem_label_refine_workspace_floats": c_int64, "uem_label_refine_select_workspace_bytes": c_int64, "uem_stem_conv_wgrad_workspace_floats": c_int64, "uem_pcl_workspace_floats": c_int64,
-            "uem_loss_workspace_floats": c_int64, "uem_layernorm_workspace_floats": c_int64}
+            "uem_loss_workspace_floats": c_int64, "uem_layernorm_workspace_floats": c_int64,
+            "uem_multi_norm_workspace_doubles": c_int64}
 
 # compile-time constants mirrored from the header
 UEM_MAX_CLASSES = 16
 UEM_PROTO_SPLIT = 256
 UEM_NORM_BLOCKS = 1024
+UEM_MULTI_BLOCKS = 8192
 CONV_IN_AFFINE, CONV_IN_RELU, CONV_ACCUMULATE, CONV_TRANSPOSED = 1, 2, 4, 8
 CONV_PREC_BF16 = 32
 LN_BF16, LN_PARAM_BF16 = 1, 2
