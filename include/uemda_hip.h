@@ -502,6 +502,30 @@ int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma, const void
 int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const void* gamma, const float* mean, const float* rstd,
                       void* dx, void* dgamma, void* dbeta, float* workspace, int64_t rows, int C, int flags, void* stream);
 
+/* ---- products grouped by expert (class, domain), ragged sizes -------------------------------------------------------------------
+ * Rows [offsets[g], offsets[g + 1]) of x / y belong to group g; offsets[G + 1] on the DEVICE, int32 (int64 with UEM_GROUPED_OFFSETS_64),
+ * not decreasing; an entry below one in front of it counts as that one, entries are clamped to [0, T].  Rows of no group: y = dx = 0.
+ *   fwd    y[r]  = W_g x[r] (+ bias_g)       x [T][K], W [G][N][K], bias [G][N] or NULL, y [T][N] dense
+ *   dgrad  dx[r] = W_g^T dy[r]               dx [T][K] dense
+ *   wgrad  dW_g  = sum_r dy[r] x[r]^T, db_g = sum_r dy[r]; WRITTEN, zeros for an empty group; dw or db may be NULL
+ * x, W, dy (and y, dx) are fp32, or bf16 with UEM_GROUPED_BF16; dW has their type, or fp32 with UEM_GROUPED_OUT_F32 (a bf16 product for an
+ * fp32 master weight); bias / db are fp32, or bf16 with UEM_GROUPED_BIAS_BF16.  *_ld: row strides in ELEMENTS; rows of the operands must
+ * begin on 16-byte boundaries and be followed by zeros up to the next one (whatever their stride holds beyond it) -- uem_grouped_pad copies
+ * rows of any length to such a stride.  No group is read beyond its
+ * rows, sums run in a fixed order.                                                                                                */
+#define UEM_GROUPED_BF16 1
+#define UEM_GROUPED_OUT_F32 2
+#define UEM_GROUPED_BIAS_BF16 4
+#define UEM_GROUPED_OFFSETS_64 8
+int uem_grouped_pad(const void* src, int64_t src_ld, void* dst, int dst_ld, int cols, int64_t rows, int flags, void* stream);
+int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void* bias, void* y, const void* offsets, int T, int G, int K, int N,
+                    int flags, void* stream);
+int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w_ld, void* dx, const void* offsets, int T, int G, int K, int N, int flags,
+                      void* stream);
+int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N);
+int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x_ld, void* dw, void* db, float* workspace, const void* offsets, int T, int G,
+                      int K, int N, int flags, void* stream);
+
 /* ---- global norm over many tensors, and clipping ------------------------------------------------------------------------------
  * ptrs / numels / bf16 are HOST arrays of `count` entries (read before the call returns): device address, elements, 1 = bf16 or 0 = fp32
  * of each tensor; a tensor may begin at any element and may be empty.  norm_type 2: sqrt of the sum of squares (summed in 64 bits, in a

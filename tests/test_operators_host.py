@@ -79,3 +79,29 @@ def test_gradient_norm_refusals():
     ptrs[0] = 0
     assert lib.uem_multi_norm(*args, b"\0\0", 2, 2, 16, 16, None) == -1
     assert lib.uem_multi_norm_workspace_doubles(3) == _lib.UEM_MULTI_BLOCKS + 6
+
+
+def test_grouped_linear_refusals():
+    from uemda_amd.grouped import GroupedLinear, grouped_linear
+    x, w, off = torch.zeros(6, 8), torch.zeros(2, 4, 8), torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(UemError, match="MI355X"):
+        grouped_linear(x, w, off)
+    for bad, text in (((x[0], w, off), "expected x"), ((x, w[0], off), "expected x"), ((x, torch.zeros(2, 4, 9), off), "expected x"),
+                      ((x, torch.zeros(0, 4, 8), off), "expected x"), ((x.half(), w.half(), off), "float32"),
+                      ((x, w.bfloat16(), off), "float32"), ((x, w, off[:2]), "offsets"), ((x, w, off.float()), "offsets"),
+                      ((x, w, off, torch.zeros(2, 5)), "bias"), ((x, w, off, torch.zeros(2, 4).half()), "bias"), ((x, w, [0, 1, 2]), "tensor")):
+        with pytest.raises(UemError, match=text):
+            grouped_linear(*bad)
+    with pytest.raises(UemError, match="positive"):
+        GroupedLinear(0, 8, 8)
+    lib = _lib.load()
+    assert lib.uem_grouped_fwd(None, 8, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1
+    assert lib.uem_grouped_fwd(16, 6, 16, 8, None, 16, 16, 4, 2, 6, 8, 0, None) == -1 and b"16-byte" in lib.uem_last_error()
+    assert lib.uem_grouped_fwd(24, 8, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1
+    assert lib.uem_grouped_fwd(16, 4, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1 and b"shorter" in lib.uem_last_error()
+    assert lib.uem_grouped_fwd(16, 8, 16, 8, None, 16, 16, 1 << 30, 2, 8, 8, 0, None) == -1
+    assert lib.uem_grouped_dgrad(16, 8, 16, 8, 16, 16, 4, 2, 8, 8, 64, None) == -1
+    assert lib.uem_grouped_wgrad(16, 8, 16, 8, 16, 16, None, 16, 4, 2, 8, 8, 0, None) == -1
+    assert lib.uem_grouped_pad(16, 4, 16, 8, 6, 4, 0, None) == -1
+    for T, G, K, N in ((1, 1, 1, 1), (100, 3, 5, 7), (1 << 20, 64, 2048, 2048)):
+        assert lib.uem_grouped_wgrad_workspace_floats(T, G, K, N) >= (T // 512 + G) * N

@@ -150,6 +150,11 @@ SIGNATURES = {
     "uem_multi_norm_workspace_doubles": [I],
     "uem_multi_norm": [P, P, P, I, I, P, P, P],
     "uem_multi_clip": [P, P, P, I, I, P, P, F, P],
+    "uem_grouped_pad": [P, L, P, I, I, L, I, P],
+    "uem_grouped_fwd": [P, I, P, I, P, P, P, I, I, I, I, I, P],
+    "uem_grouped_dgrad": [P, I, P, I, P, P, I, I, I, I, I, P],
+    "uem_grouped_wgrad_workspace_floats": [I, I, I, I],
+    "uem_grouped_wgrad": [P, I, P, I, P, P, P, P, I, I, I, I, I, P],
     "uem_comm_unique_id": [P],
     "uem_comm_init": [POINTER(c_void_p), P, I, I],
     "uem_allreduce_flat": [P, P, L, P],
@@ -160,7 +165,7 @@ SIGNATURES = {
 _RESTYPE = {"uem_last_error": c_char_p, "uem_bn_workspace_floats": c_int64,
             "uem_label_refine_workspace_floats": c_int64, "uem_label_refine_select_workspace_bytes": c_int64, "uem_stem_conv_wgrad_workspace_floats": c_int64, "uem_pcl_workspace_floats": c_int64,
             "uem_loss_workspace_floats": c_int64, "uem_layernorm_workspace_floats": c_int64,
-            "uem_multi_norm_workspace_doubles": c_int64}
+            "uem_multi_norm_workspace_doubles": c_int64, "uem_grouped_wgrad_workspace_floats": c_int64}
 
 # compile-time constants mirrored from the header
 UEM_MAX_CLASSES = 16
@@ -170,6 +175,7 @@ UEM_MULTI_BLOCKS = 8192
 CONV_IN_AFFINE, CONV_IN_RELU, CONV_ACCUMULATE, CONV_TRANSPOSED = 1, 2, 4, 8
 CONV_PREC_BF16 = 32
 LN_BF16, LN_PARAM_BF16 = 1, 2
+GROUPED_BF16, GROUPED_OUT_F32, GROUPED_BIAS_BF16, GROUPED_OFFSETS_64 = 1, 2, 4, 8
 PREP_TRANSPOSE, PREP_WINO2, PREP_WINO2_T, PREP_WINO4, PREP_WINO4_T, PREP_STEM_PACK, PREP_TRANSPOSE_BF16 = range(7)
 
 
