@@ -6,7 +6,7 @@
 // Rows in front of offsets[0] and behind offsets[G] belong to no group: their y and dx are zeros and they enter no gradient.
 //
 // Matrix-bound (2 T K N flops each) once a group has some hundred rows, bound by reading W below.  One kernel serves the three: an
-// operand tile travels global -> LDS by 16-byte LDS-DMA as 128 bytes of the reduction index per tile row, two stages, one barrier a stage;
+// operand tile travels global -> LDS by 16-byte LDS-DMA, 64 bytes of the reduction index per tile row a stage, four stages;
 // where the reduction index is the SLOW one in memory (W in the data gradient, both operands of the weight gradient) the image is kept as
 // it sits in memory and read transposed: bf16 by ds_read_b64_tr_b16, fp32 by consecutive ds_read_b32.  Both kinds are XOR-swizzled in
 // 16-byte chunks on the source address so that a read covers all banks.  Buffer descriptors that end with the group's last row (and
@@ -139,15 +139,16 @@ __device__ __forceinline__ int xcd_item(int n) {
 }
 
 // ---- operand images -------------------------------------------------------------------------------------------------------------------
-// KC (reduction index contiguous in memory): [R rows][128 bytes], chunk c of row r in slot c ^ ((r >> 1) & 7): the 16 rows a quarter-wave
+// A stage holds 64 bytes of the reduction index (32 bf16, 16 fp32) of every tile row.
+// KC (reduction index contiguous in memory): [R rows][64 bytes], chunk c of row r in slot c ^ ((r >> 2) & 3): the 16 rows a quarter-wave
 // of ds_read_b128 touches fall on 16 different 16-byte slots of the 256-byte bank row.
-// KS (reduction index slow): [128 / ES reduction rows][R columns]; bf16: chunk c of row r in slot c ^ ((r & 3) << 2): the four rows of a
+// KS (reduction index slow): [64 / ES reduction rows][R columns]; bf16: chunk c of row r in slot c ^ ((r & 3) << 2): the four rows of a
 // transposing read fall on the four quarters of the bank row.
 template <int ES> __device__ __forceinline__ int ks_swz(int row) { return ES == 2 ? (row & 3) << 2 : 0; }
 
 template <typename T, bool KS, int R, int NW>
 struct Loader {
-    static constexpr int ES = sizeof(T), PIECES = R / 8, IPW = PIECES / NW, ROWB = R * ES, LPR = ROWB / 16, RPP = 1024 / ROWB > 0 ? 1024 / ROWB : 1, BK = 128 / ES;
+    static constexpr int ES = sizeof(T), PIECES = R / 16, IPW = PIECES / NW, ROWB = R * ES, LPR = ROWB / 16, RPP = 1024 / ROWB > 0 ? 1024 / ROWB : 1;
     static_assert(PIECES % NW == 0, "whole pieces a wave");
     unsigned off[IPW];
     int kc[IPW];                                  // KC: first reduction index of the lane's chunk
@@ -157,7 +158,7 @@ struct Loader {
         for (int j = 0; j < IPW; ++j) {
             const int q = j * NW + wave;
             if (!KS) {
-                const int row = q * 8 + (lane >> 3), ch = (lane & 7) ^ ((row >> 1) & 7);
+                const int row = q * 16 + (lane >> 2), ch = (lane & 3) ^ ((row >> 2) & 3);
                 off[j] = (unsigned)(row * bytes + ch * 16);
                 kc[j] = ch * (16 / ES);
             } else {
@@ -181,8 +182,8 @@ template <typename T, bool KS, int R> struct Frag;
 template <int R> struct Frag<bf16_t, false, R> {
     bf16x8 v;
     __device__ __forceinline__ void load(const char* img, int r0, int ks, int lane) {
-        const int r = r0 + (lane & 31), ch = (2 * ks + (lane >> 5)) ^ ((r >> 1) & 7);
-        v = *reinterpret_cast<const bf16x8*>(img + r * 128 + ch * 16);
+        const int r = r0 + (lane & 31), ch = (2 * ks + (lane >> 5)) ^ ((r >> 2) & 3);
+        v = *reinterpret_cast<const bf16x8*>(img + r * 64 + ch * 16);
     }
 };
 template <int R> struct Frag<bf16_t, true, R> {
@@ -200,8 +201,8 @@ template <int R> struct Frag<bf16_t, true, R> {
 template <int R> struct Frag<float, false, R> {
     f32x4 v;
     __device__ __forceinline__ void load(const char* img, int r0, int ks, int lane) {
-        const int r = r0 + (lane & 31), ch = (2 * ks + (lane >> 5)) ^ ((r >> 1) & 7);
-        v = *reinterpret_cast<const f32x4*>(img + r * 128 + ch * 16);
+        const int r = r0 + (lane & 31), ch = (2 * ks + (lane >> 5)) ^ ((r >> 2) & 3);
+        v = *reinterpret_cast<const f32x4*>(img + r * 64 + ch * 16);
     }
 };
 template <int R> struct Frag<float, true, R> {
@@ -221,14 +222,20 @@ template <typename FA, typename FB> __device__ __forceinline__ void mma(const FA
 
 __device__ __forceinline__ unsigned bf_bits(float f) { return (unsigned)__builtin_bit_cast(unsigned short, (__bf16)f); }
 
-#define GG_SYNC()                                                   \
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");     \
-    __builtin_amdgcn_s_barrier();                                   \
-    asm volatile("" ::: "memory")
+// own LDS-DMA pieces but the last N, and own LDS accesses, complete; then everybody's
+template <int N> __device__ __forceinline__ void gg_wait() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void gg_barrier() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 
+// Four stages: the pieces of stage t + 3 leave while stage t is computed on, a wait is for pieces that left two stages ago.
+// PP (eight waves, one block a CU): the two waves of a SIMD take turns -- while one feeds the matrix cores from registers, the other reads
+// its next fragments and sends pieces off, a barrier between the turns.  With the waves in step both wait for LDS at the same time.
 template <typename T, int FORM, int BM, int BN, int WGM, int WGN>
 __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p) {
-    constexpr int ES = sizeof(T), NW = WGM * WGN, MT = BM / WGM / 32, NT = BN / WGN / 32, BK = 128 / ES, SB = (BM + BN) * 128;
+    constexpr int ES = sizeof(T), NW = WGM * WGN, MT = BM / WGM / 32, NT = BN / WGN / 32, BK = 64 / ES, SB = (BM + BN) * 64, NST = 4;
+    constexpr bool PP = NW == 8;
     constexpr bool AKS = FORM == WGRAD, BKS = FORM != FWD;
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -277,43 +284,66 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     int arem = rows, brem = FORM == FWD ? (p.N - c0 < BN ? p.N - c0 : BN) : FORM == DGRAD ? p.N : rows;    // rows left of a and b
     int q = 0;                                                                 // the next step to issue
 
-    auto step = [&](char* __restrict__ fill, const char* __restrict__ use, const bool do_issue, const bool do_phase) {
-        if (do_issue) {
-            const int na = AKS && arem > BK ? BK : arem, nb = BKS && brem > BK ? BK : brem;
-            const i32x4 ra = rsrc(pa, (unsigned)((na - 1) * p.lda) + acols), rb = rsrc(pb, (unsigned)((nb - 1) * p.ldb) + bcols);
-            la.issue(ra, fill, wave, (unsigned)q * 128u, q * BK, red);
-            lb.issue(rb, fill + BM * 128, wave, (unsigned)q * 128u, q * BK, red);
-            if (AKS) { pa += BK * p.lda; arem -= BK; }
-            if (BKS) { pb += BK * p.ldb; brem -= BK; }
-            ++q;
-        }
-        if (!do_phase) return;
-        // fragments one reduction step ahead of the MFMAs, and no further: the accumulators and two sets of fragments fill the registers
-        Frag<T, AKS, BM> a[2][MT];
-        Frag<T, BKS, BN> b[2][NT];
+    constexpr int IPW = Loader<T, AKS, BM, NW>::IPW + Loader<T, BKS, BN, NW>::IPW;
+    auto issue = [&](char* __restrict__ fill) {                                // steps past the end fetch zeros: the counts of the waits hold
+        const int na = AKS && arem > BK ? BK : arem, nb = BKS && brem > BK ? BK : brem;
+        const i32x4 ra = rsrc(pa, na > 0 ? (unsigned)((na - 1) * p.lda) + acols : 0u), rb = rsrc(pb, nb > 0 ? (unsigned)((nb - 1) * p.ldb) + bcols : 0u);
+        la.issue(ra, fill, wave, (unsigned)q * 64u, q * BK, red);
+        lb.issue(rb, fill + BM * 64, wave, (unsigned)q * 64u, q * BK, red);
+        if (AKS) { pa += BK * p.lda; arem -= BK; }
+        if (BKS) { pb += BK * p.ldb; brem -= BK; }
+        ++q;
+    };
+    Frag<T, AKS, BM> fa[2][MT];
+    Frag<T, BKS, BN> fb[2][NT];
+    // one function with the stage being refilled and the stage being read as __restrict__ pointers: that is what tells the compiler that
+    // the reads do not depend on the LDS-DMA in flight (it would wait for all of it in front of the first read)
+    auto stage = [&](char* __restrict__ fill, const char* __restrict__ use) {
         auto fetch = [&](const int ks) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) a[ks & 1][i].load(use, wm + i * 32, ks, lane);
+            for (int i = 0; i < MT; ++i) fa[ks][i].load(use, wm + i * 32, ks, lane);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) b[ks & 1][j].load(use + BM * 128, wn + j * 32, ks, lane);
+            for (int j = 0; j < NT; ++j) fb[ks][j].load(use + BM * 64, wn + j * 32, ks, lane);
         };
-        fetch(0);
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks) {
-            if (ks < 3) fetch(ks + 1);
+        auto multiply = [&](const int ks) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) mma(a[ks & 1][i], b[ks & 1][j], acc[i][j], T{});
+                for (int j = 0; j < NT; ++j) mma(fa[ks][i], fb[ks][j], acc[i][j], T{});
+        };
+        if (PP) {
+            fetch(0);
+            fetch(1);
+            issue(fill);
+            gg_wait<2 * IPW>();
+            gg_barrier();
+            __builtin_amdgcn_s_setprio(1);
+            multiply(0);
+            multiply(1);
+            __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
+            gg_barrier();
+        } else {
+            gg_wait<2 * IPW>();
+            gg_barrier();
+            issue(fill);
+            fetch(0);
+            fetch(1);
+            multiply(0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(1);
         }
     };
     if (steps > 0) {
-        step(smem, smem + SB, true, false);
-        for (int t = 0; t < steps; ++t) {
-            GG_SYNC();
-            step(smem + ((t + 1) & 1) * SB, smem + (t & 1) * SB, t + 1 < steps, true);
+#pragma unroll
+        for (int t = 0; t < NST - 1; ++t) issue(smem + t * SB);
+        if (PP) {
+            gg_wait<2 * IPW>();
+            gg_barrier();
+            if (wave >= NW / 2) gg_barrier();
         }
+        for (int t = 0; t < steps; ++t) stage(smem + ((t + NST - 1) % NST) * SB, smem + (t % NST) * SB);
+        if (PP && wave < NW / 2) gg_barrier();
     }
 
     // ---- results: MFMA column = lane & 31, row = (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
@@ -337,8 +367,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     const bool o16 = partial ? false : p.out16;
     char* const out = partial ? (char*)p.part : p.out;
     const bool vec = partial ? (p.K & 3) == 0 : p.vec;
-    GG_SYNC();                                                                 // everybody has read the last stage: its memory stages results
-    constexpr int STG = 2 * SB / NW;
+    gg_wait<0>();                                                              // everybody has read the last stage and nothing is on its way:
+    gg_barrier();                                                              // the stages' memory takes the results
+    constexpr int STG = NST * SB / NW;
     static_assert(STG >= 32 * NT * 32 * 4, "a wave's 32 result rows");
     char* const mine = smem + wave * STG;
     auto leave = [&](auto out_t) {
@@ -470,7 +501,7 @@ __global__ __launch_bounds__(256) void grouped_pad_kernel(const T* __restrict__ 
 
 template <typename T, int FORM, int BM, int BN, int WGM, int WGN>
 void go(const GgP& p, int64_t items, hipStream_t st) {
-    constexpr int LDS = 2 * (BM + BN) * 128;
+    constexpr int LDS = 4 * (BM + BN) * 64;
     auto k = grouped_kernel<T, FORM, BM, BN, WGM, WGN>;
     if (!uem_allow_lds((const void*)k, LDS)) return;
     k<<<(unsigned)items, 64 * WGM * WGN, LDS, st>>>(p);
@@ -480,11 +511,11 @@ void go(const GgP& p, int64_t items, hipStream_t st) {
 int64_t most_tiles(int T, int G, int bm) { return T / bm + (int64_t)G + 2; }
 
 // Tile of the forward and the data gradient.  256 x 256 moves the fewest operand bytes a flop; it needs enough tiles to fill the CUs and
-// groups that fill it.  32 x 128 is for groups of a few rows, where the weight's bytes are what counts.
+// groups that fill it.  64 x 128 is for groups of a few rows, where the weight's bytes are what counts.
 int tile_rows(int T, int G, int width) {
     const int64_t per = uem_cdiv(T, G);
     if (per >= 192 && (uem_cdiv(T, 256) + G / 2) * uem_cdiv(width, 256) >= 192) return 256;
-    return per >= 48 ? 128 : 32;
+    return per >= 80 ? 128 : 64;
 }
 // rows of a weight-gradient item: all of them where the groups' tiles fill the chip anyway, else so that it is filled
 int wgrad_chunk(int T, int G, int N, int K, int bm) {
@@ -502,7 +533,7 @@ int launch_rows(const GgP& p, const char* what, hipStream_t st) {
     UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than a launch takes", what, (long long)items);
     if (bm == 256) go<T, FORM, 256, 256, 2, 4>(p, items, st);
     else if (bm == 128) go<T, FORM, 128, 128, 2, 2>(p, items, st);
-    else go<T, FORM, 32, 128, 1, 4>(p, items, st);
+    else go<T, FORM, 64, 128, 1, 4>(p, items, st);
     return uem_check_launch(what);
 }
 
