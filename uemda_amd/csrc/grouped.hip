@@ -6,15 +6,14 @@
 // Rows in front of offsets[0] and behind offsets[G] belong to no group: their y and dx are zeros and they enter no gradient.
 //
 // Matrix-bound (2 T K N flops each) once a group has some hundred rows, bound by reading W below.  One kernel serves the three: an
-// operand tile travels global -> LDS by 16-byte LDS-DMA, 64 bytes of the reduction index per tile row a stage, four stages;
+// operand tile travels global -> LDS by 16-byte LDS-DMA, 64 bytes of the reduction index per tile row a stage, five stages;
 // where the reduction index is the SLOW one in memory (W in the data gradient, both operands of the weight gradient) the image is kept as
 // it sits in memory and read transposed: bf16 by ds_read_b64_tr_b16, fp32 by consecutive ds_read_b32.  Both kinds are XOR-swizzled in
 // 16-byte chunks on the source address so that a read covers all banks.  Buffer descriptors that end with the group's last row (and
 // offsets beyond them for columns past the end) supply the zeros of every ragged edge: no row of another group is ever read.
 // Products are exact in the fp32 accumulators (bf16) or fp32 MFMA (fp32); bf16 results are rounded once.
 //
-// Nothing is read on the host: a block finds its tile by scanning the offsets (a wave's prefix sums, ~0.5 us for up to 62 groups), the grid
-// is the most tiles T rows in G groups can make.  Offsets are clamped to [0, T] and to the largest one in front of them, so that any
+// Nothing is read on the host: a block finds its tiles by prefix sums over the offsets, 64 groups to a wave, kept in registers.  Offsets are clamped to [0, T] and to the largest one in front of them, so that any
 // contents give disjoint groups inside the tensors.
 #include "common.h"
 
@@ -61,11 +60,6 @@ __device__ __forceinline__ i32x4 rsrc(const char* p, unsigned bytes) {
 }
 
 // ---- which rows ---------------------------------------------------------------------------------------------------------------------
-// Segments of the rows: ALL: 0 = the rows in front of the first group, 1 .. G the groups, G + 1 the rows behind the last; !ALL: the groups.
-struct Seg {
-    int seg, row0, rows, tile;                    // segment, its first row and length, tile within it
-    int total, before, nslots, slot;              // tiles in all; tiles before this segment; partial-sum slots in all, this segment's first
-};
 __device__ __forceinline__ int gg_offset(const GgP& p, int i) {
     int64_t o = p.off64 ? ((const int64_t*)p.offsets)[i] : (int64_t)((const int*)p.offsets)[i];
     o = o < 0 ? 0 : o;
@@ -81,58 +75,71 @@ __device__ __forceinline__ int scan_max(int v, int lane) {
     for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v = u > v ? u : v; }
     return v;
 }
-// Tiles of `bm` rows (!ALL: an empty group still has one, which writes its zeros).  Pass 0 counts them; `want` (a function of the count:
-// which tile this block takes, < 0 for none) is then found in pass 1 -- the same pass where all segments fit one wave.  Slots are counted
-// over groups of several tiles only.
-template <bool ALL, typename Want>
-__device__ __forceinline__ bool find_tile(const GgP& p, int bm, Want want, Seg& s) {
-    const int lane = threadIdx.x & 63, nseg = ALL ? p.G + 2 : p.G, chunks = (nseg + 63) >> 6;
-    int target = -1;
-    s.total = s.nslots = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        int edge = ALL ? 0 : gg_offset(p, 0), tiles = 0, slots = 0;
-        for (int c = 0; c < chunks; ++c) {
-            const int v = c * 64 + lane;
-            int end = v < nseg ? (ALL ? (v <= p.G ? gg_offset(p, v) : p.T) : gg_offset(p, v + 1)) : 0;
-            end = scan_max(end > edge ? end : edge, lane);
-            const int up = __shfl_up(end, 1, 64), begin = lane == 0 ? edge : up;
-            const int len = end - begin;
-            int nt = v < nseg ? (len + bm - 1) / bm : 0;
-            if (!ALL && v < nseg && nt == 0) nt = 1;
-            const int sum = scan_add(nt, lane) + tiles, ns = ALL ? 0 : scan_add(nt > 1 ? nt : 0, lane) + slots;
-            if (pass == 1 || chunks == 1) {
-                if (chunks == 1) {
-                    s.total = __shfl(sum, 63, 64);
-                    s.nslots = ALL ? 0 : __shfl(ns, 63, 64);
-                    target = want(s.total);
-                    if (target < 0) return false;
-                }
-                const unsigned long long hit = __ballot(sum > target);
-                if (hit != 0) {
-                    const int l = __builtin_ctzll(hit);
-                    s.seg = c * 64 + l;
-                    s.before = __shfl(sum - nt, l, 64);
-                    s.tile = target - s.before;
-                    s.row0 = __shfl(begin, l, 64);
-                    s.rows = __shfl(len, l, 64);
-                    s.slot = ALL ? 0 : __shfl(ns - (nt > 1 ? nt : 0), l, 64);
-                    return true;
-                }
-            }
-            edge = __shfl(end, 63, 64);
-            tiles = __shfl(sum, 63, 64);
-            slots = ALL ? 0 : __shfl(ns, 63, 64);
-        }
-        if (pass == 0) {
-            s.total = tiles;
-            s.nslots = slots;
-            target = want(s.total);
-            if (target < 0) return false;
-        }
+__device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+
+// The groups cut into tiles of `bm` rows, 64 groups at a time, one a lane.  ONE: an empty group still has a tile (which writes its zeros).
+// `slot`: groups of several tiles take that many slots for partial sums, the others none.
+struct Tile { int group, row0, rows, tile, before, slot; };       // rows: of the whole group; before: tiles of the groups in front of it
+template <bool ONE>
+struct Groups {
+    int begin, len, nt, tiles, slots;             // of the lane's group; tiles, slots: up to and with it
+    int loaded;                                   // which 64 groups the lanes hold
+    int first, last, total, nslots;               // rows of all groups: [first, last); tiles and slots in all
+    __device__ __forceinline__ void load(const GgP& p, int bm, int chunk, int lane, int& edge, int& ntiles, int& nslot) {
+        const int v = chunk * 64 + lane;
+        int end = v < p.G ? gg_offset(p, v + 1) : 0;
+        end = scan_max(end > edge ? end : edge, lane);
+        const int up = __shfl_up(end, 1, 64);
+        begin = lane == 0 ? edge : up;
+        len = end - begin;
+        nt = v < p.G ? (len + bm - 1) / bm : 0;
+        if (ONE && v < p.G && nt == 0) nt = 1;
+        tiles = scan_add(nt, lane) + ntiles;
+        slots = ONE ? scan_add(nt > 1 ? nt : 0, lane) + nslot : 0;
+        loaded = chunk;
+        edge = lane_value(end, 63);
+        ntiles = lane_value(tiles, 63);
+        nslot = ONE ? lane_value(slots, 63) : 0;
     }
-    return false;
-}
-// Blocks go to the eight XCDs in turn: each gets one contiguous run of the n items, neighbours share their operand tiles in its L2.
+    __device__ __forceinline__ void init(const GgP& p, int bm, int lane) {
+        first = __builtin_amdgcn_readfirstlane(gg_offset(p, 0));
+        last = first;
+        total = nslots = 0;
+        for (int c = 0; c * 64 < p.G; ++c) load(p, bm, c, lane, last, total, nslots);
+    }
+    __device__ __forceinline__ bool pick(int l, Tile& t) const {
+        t.group = loaded * 64 + l;
+        t.before = lane_value(tiles, l) - lane_value(nt, l);
+        t.row0 = lane_value(begin, l);
+        t.rows = lane_value(len, l);
+        t.slot = ONE ? lane_value(slots, l) - (lane_value(nt, l) > 1 ? lane_value(nt, l) : 0) : 0;
+        return true;
+    }
+    // tile number `target` < total
+    __device__ __forceinline__ Tile find(const GgP& p, int bm, int lane, int target) {
+        Tile t{};
+        if (p.G > 64) {                                                        // walk the groups 64 at a time again
+            int edge = first, ntiles = 0, nslot = 0;
+            for (int c = 0; c * 64 < p.G; ++c) {
+                load(p, bm, c, lane, edge, ntiles, nslot);
+                if (ntiles > target) break;
+            }
+        }
+        pick(__builtin_ctzll(__ballot(tiles > target)), t);
+        t.tile = target - t.before;
+        return t;
+    }
+    // the tiles of group `g`
+    __device__ __forceinline__ Tile of(const GgP& p, int bm, int lane, int g, int& n) {
+        Tile t{};
+        int edge = __builtin_amdgcn_readfirstlane(gg_offset(p, 0)), ntiles = 0, nslot = 0;
+        for (int c = 0; c * 64 <= g; ++c) load(p, bm, c, lane, edge, ntiles, nslot);
+        pick(g & 63, t);
+        n = lane_value(nt, g & 63);
+        return t;
+    }
+};
+// Blocks go to the eight XCDs in turn: each XCD gets one contiguous run of the n items, neighbours share operand tiles in its L2.
 __device__ __forceinline__ int xcd_item(int n) {
     const int x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rem = n & 7;
     return i < per + (x < rem ? 1 : 0) ? x * per + (x < rem ? x : rem) + i : -1;
@@ -168,12 +175,10 @@ struct Loader {
             }
         }
     }
-    __device__ __forceinline__ void issue(const i32x4 rs, char* img, int wave, unsigned step_bytes, int k0, int klen) const {
-#pragma unroll
-        for (int j = 0; j < IPW; ++j) {
-            const unsigned o = KS ? off[j] : (k0 + kc[j] < klen ? off[j] + step_bytes : GG_OOB);
-            uem_raw_buffer_load_lds(rs, (lds_u32p)(img + (j * NW + wave) * 1024), 16, (int)o, 0, 0, 0);
-        }
+    // piece j of stage `q` of a reduction of `red`
+    __device__ __forceinline__ void issue(int j, const i32x4 rs, char* img, int wave, int q, int red) const {
+        const unsigned o = KS ? off[j] : (q * (64 / ES) + kc[j] < red ? off[j] + (unsigned)q * 64u : GG_OOB);
+        uem_raw_buffer_load_lds(rs, (lds_u32p)(img + (j * NW + wave) * 1024), 16, (int)o, 0, 0, 0);
     }
 };
 
@@ -229,38 +234,105 @@ __device__ __forceinline__ void gg_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// Four stages: the pieces of stage t + 3 leave while stage t is computed on, a wait is for pieces that left two stages ago.
+// One tile a block.  Five stages: while stage t is computed on, a KS operand's pieces of stage t + 4 leave, a KC operand's of stages t + 3 and
+// t + 4 together if t is odd -- the two halves of every 128-byte line one after the other, or the line travels from L2 twice (65536 x 2048 ->
+// 2048 in 32 groups, forward: 545 us stage by stage, 515 in pairs; KS operands in pairs lose: weight gradient 488 against 529).
 // PP (eight waves, one block a CU): the two waves of a SIMD take turns -- while one feeds the matrix cores from registers, the other reads
 // its next fragments and sends pieces off, a barrier between the turns.  With the waves in step both wait for LDS at the same time.
+// The MFMA's rows are the output's COLUMNS (its A operand is tile b): a lane ends up with four neighbouring columns of one row.
 template <typename T, int FORM, int BM, int BN, int WGM, int WGN>
 __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p) {
-    constexpr int ES = sizeof(T), NW = WGM * WGN, MT = BM / WGM / 32, NT = BN / WGN / 32, BK = 64 / ES, SB = (BM + BN) * 64, NST = 4;
-    constexpr bool PP = NW == 8;
-    constexpr bool AKS = FORM == WGRAD, BKS = FORM != FWD;
+    constexpr int ES = sizeof(T), NW = WGM * WGN, MT = BM / WGM / 32, NT = BN / WGN / 32, BK = 64 / ES, SB = (BM + BN) * 64, NST = 5;
+    constexpr bool PP = NW == 8, AKS = FORM == WGRAD, BKS = FORM != FWD;
+    using LA = Loader<T, AKS, BM, NW>;
+    using LB = Loader<T, BKS, BN, NW>;
+    constexpr int FLIGHT = LA::IPW * (AKS ? 3 : 2) + LB::IPW * (BKS ? 3 : 2);
+    constexpr int ROWB = NT * 64, CPR = ROWB / 16;                             // bf16 results: bytes and 16-byte chunks of a wave's row
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-
-    // ---- this block's tile
+    const int bm = FORM == WGRAD ? p.chunk : BM;                               // feature rows of a tile / of a chunk
     const int width = FORM == FWD ? p.N : p.K;                                 // output columns
     const int ct = (width + BN - 1) / BN, rt = FORM == WGRAD ? (p.N + BM - 1) / BM : 1;
-    Seg s;
-    int item = -1;
-    if (!find_tile<FORM != WGRAD>(p, FORM == WGRAD ? p.chunk : BM, [&](int total) {
-            item = xcd_item(total * ct * rt);
-            return item < 0 ? -1 : item / (ct * rt);
-        }, s)) return;
-    s.seg = __builtin_amdgcn_readfirstlane(s.seg);
-    s.row0 = __builtin_amdgcn_readfirstlane(s.row0);
-    s.rows = __builtin_amdgcn_readfirstlane(s.rows);
-    s.tile = __builtin_amdgcn_readfirstlane(s.tile);
-    const int within = item % (ct * rt), c0 = (within % ct) * BN, n0 = (within / ct) * BM;      // n0: first row of W (WGRAD)
-    const bool none = FORM != WGRAD && (s.seg == 0 || s.seg == p.G + 1);
-    const int g = FORM == WGRAD ? s.seg : s.seg - 1;
-    const int r0 = s.row0 + s.tile * (FORM == WGRAD ? p.chunk : BM);           // first feature row of the tile / of the chunk
-    int rows = s.rows - s.tile * (FORM == WGRAD ? p.chunk : BM);               // feature rows of it
-    rows = rows < 0 ? 0 : rows < (FORM == WGRAD ? p.chunk : BM) ? rows : (FORM == WGRAD ? p.chunk : BM);
+    Groups<FORM == WGRAD> groups;
+    groups.init(p, bm, lane);
 
+    // ---- rows of no group: zeros
+    if (FORM != WGRAD) {
+        const int head = groups.first, zeros = head + p.T - groups.last;
+        for (int z = blockIdx.x; z < zeros; z += gridDim.x) {
+            const int64_t at = (int64_t)(z < head ? z : groups.last + z - head) * p.ldo;
+            if (p.vec) {
+                const int n = p.out16 ? 8 : 4;
+                for (int c = tid * n; c < width; c += 64 * NW * n) *reinterpret_cast<uint4*>(p.out + (at + c) * (p.out16 ? 2 : 4)) = make_uint4(0, 0, 0, 0);
+            } else {
+                for (int c = tid; c < width; c += 64 * NW)
+                    if (p.out16) reinterpret_cast<bf16_t*>(p.out)[at + c] = 0;
+                    else reinterpret_cast<float*>(p.out)[at + c] = 0.f;
+            }
+        }
+    }
+    const int item = xcd_item(groups.total * ct * rt);
+    if (item < 0) return;
+
+    // ---- the tile
+    const Tile tl = groups.find(p, bm, lane, item / (ct * rt));
+    const int within = item % (ct * rt), c0 = (within % ct) * BN, n0 = (within / ct) * BM;      // n0: first row of W (WGRAD)
+    const int r0 = tl.row0 + tl.tile * bm;
+    int rows = tl.rows - tl.tile * bm;                                         // feature rows of the tile
+    rows = rows < 0 ? 0 : rows < bm ? rows : bm;
+    const int red = FORM == FWD ? p.K : FORM == DGRAD ? p.N : rows;            // reduction length
+    const int steps = (red + BK - 1) / BK;
+    LA la;
+    LB lb;
+    la.init(wave, lane, p.lda, n0, p.N);
+    lb.init(wave, lane, p.ldb, c0, p.K);
+    const char* pa = p.a + (int64_t)r0 * p.lda;
+    const char* pb = FORM == FWD ? p.b + ((int64_t)tl.group * p.N + c0) * p.ldb : FORM == DGRAD ? p.b + (int64_t)tl.group * p.N * p.ldb : p.b + (int64_t)r0 * p.ldb;
+    // bytes of a row, up to the 16-byte boundary behind its last element (zeros there)
+    const unsigned acols = (unsigned)((FORM == FWD ? p.K : p.N) * ES + 15) & ~15u, bcols = (unsigned)(p.K * ES + 15) & ~15u;
+    int arem = rows, brem = FORM == FWD ? (p.N - c0 < BN ? p.N - c0 : BN) : FORM == DGRAD ? p.N : rows;       // rows left of a and b
+    const int wm = (wave / WGN) * (MT * 32), wn = (wave % WGN) * (NT * 32);
+    float bias = 0.f;                                                          // of column wn + lane
+    if (FORM == FWD && p.bias != nullptr) {
+        const int c = c0 + wn + lane;
+        const int64_t i = (int64_t)tl.group * p.N + c;
+        if (lane < NT * 32 && c < p.N) bias = p.bias16 ? __uint_as_float((uint32_t)((const bf16_t*)p.bias)[i] << 16) : ((const float*)p.bias)[i];
+    }
+
+    // One operand's stage `q`, or stages `q` and `q` + 1; those past the end fetch zeros, so that the waits' counts hold
+    auto desc = [](const char* b, int rem, int64_t ld, unsigned bytes, bool ks) {
+        const int n = ks && rem > BK ? BK : rem;
+        return rsrc(b, n > 0 ? (unsigned)((n - 1) * ld) + bytes : 0u);
+    };
+    int qa = 0, qb = 0;                                                        // next stages to send off
+    auto issue_a = [&](char* __restrict__ fill0, char* __restrict__ fill1, const bool two) {
+        const i32x4 r0_ = desc(pa, arem, p.lda, acols, AKS);
+#pragma unroll
+        for (int j = 0; j < LA::IPW; ++j) {
+            la.issue(j, r0_, fill0, wave, qa, red);
+            if (two) la.issue(j, r0_, fill1, wave, qa + 1, red);
+        }
+        if (AKS) { pa += BK * p.lda; arem -= BK; }
+        qa += two ? 2 : 1;
+    };
+    auto issue_b = [&](char* __restrict__ fill0, char* __restrict__ fill1, const bool two) {
+        const i32x4 r0_ = desc(pb, brem, p.ldb, bcols, BKS);
+#pragma unroll
+        for (int j = 0; j < LB::IPW; ++j) {
+            lb.issue(j, r0_, fill0 + BM * 64, wave, qb, red);
+            if (two) lb.issue(j, r0_, fill1 + BM * 64, wave, qb + 1, red);
+        }
+        if (BKS) { pb += BK * p.ldb; brem -= BK; }
+        qb += two ? 2 : 1;
+    };
+    // in stage t: a KC operand's stages t + 3 and t + 4 if t is odd, a KS operand's stage t + 4
+    auto issue = [&](char* __restrict__ fill3, char* __restrict__ fill4, const bool odd) {
+        if (AKS) issue_a(fill4, fill4, false);
+        else if (odd) issue_a(fill3, fill4, true);
+        if (BKS) issue_b(fill4, fill4, false);
+        else if (odd) issue_b(fill3, fill4, true);
+    };
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -268,37 +340,11 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-    const int wm = (wave / WGN) * (MT * 32), wn = (wave % WGN) * (NT * 32);
-
-    // ---- operands: where they begin, how far they reach, how long the reduction is
-    const int red = FORM == FWD ? p.K : FORM == DGRAD ? p.N : rows;            // reduction length
-    const int steps = none ? 0 : (red + BK - 1) / BK;
-    Loader<T, AKS, BM, NW> la;
-    Loader<T, BKS, BN, NW> lb;
-    la.init(wave, lane, p.lda, n0, p.N);
-    lb.init(wave, lane, p.ldb, c0, p.K);
-    const char* pa = p.a + (int64_t)r0 * p.lda;
-    const char* pb = FORM == FWD ? p.b + ((int64_t)g * p.N + c0) * p.ldb : FORM == DGRAD ? p.b + (int64_t)g * p.N * p.ldb : p.b + (int64_t)r0 * p.ldb;
-    // bytes of a row, up to the 16-byte boundary behind its last element (zeros there)
-    const unsigned acols = (unsigned)((FORM == FWD ? p.K : p.N) * ES + 15) & ~15u, bcols = (unsigned)(p.K * ES + 15) & ~15u;
-    int arem = rows, brem = FORM == FWD ? (p.N - c0 < BN ? p.N - c0 : BN) : FORM == DGRAD ? p.N : rows;    // rows left of a and b
-    int q = 0;                                                                 // the next step to issue
-
-    constexpr int IPW = Loader<T, AKS, BM, NW>::IPW + Loader<T, BKS, BN, NW>::IPW;
-    auto issue = [&](char* __restrict__ fill) {                                // steps past the end fetch zeros: the counts of the waits hold
-        const int na = AKS && arem > BK ? BK : arem, nb = BKS && brem > BK ? BK : brem;
-        const i32x4 ra = rsrc(pa, na > 0 ? (unsigned)((na - 1) * p.lda) + acols : 0u), rb = rsrc(pb, nb > 0 ? (unsigned)((nb - 1) * p.ldb) + bcols : 0u);
-        la.issue(ra, fill, wave, (unsigned)q * 64u, q * BK, red);
-        lb.issue(rb, fill + BM * 64, wave, (unsigned)q * 64u, q * BK, red);
-        if (AKS) { pa += BK * p.lda; arem -= BK; }
-        if (BKS) { pb += BK * p.ldb; brem -= BK; }
-        ++q;
-    };
     Frag<T, AKS, BM> fa[2][MT];
     Frag<T, BKS, BN> fb[2][NT];
-    // one function with the stage being refilled and the stage being read as __restrict__ pointers: that is what tells the compiler that
+    // one function with the stages being refilled and the stage being read as __restrict__ pointers: that is what tells the compiler that
     // the reads do not depend on the LDS-DMA in flight (it would wait for all of it in front of the first read)
-    auto stage = [&](char* __restrict__ fill, const char* __restrict__ use) {
+    auto stage = [&](char* __restrict__ fill3, char* __restrict__ fill4, const char* __restrict__ use, const bool odd) {
         auto fetch = [&](const int ks) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) fa[ks][i].load(use, wm + i * 32, ks, lane);
@@ -309,13 +355,15 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) mma(fa[ks][i], fb[ks][j], acc[i][j], T{});
+                for (int j = 0; j < NT; ++j) mma(fb[ks][j], fa[ks][i], acc[i][j], T{});
         };
+        // In front of stage t (PP: in stage t - 1, behind its sends) the pieces of stage t have to have landed.  Newer than the last of them
+        // are, of a KS operand, three stages' pieces and, of a KC operand, those of the pair behind its own (and, t even, its partner's last).
         if (PP) {
             fetch(0);
             fetch(1);
-            issue(fill);
-            gg_wait<2 * IPW>();
+            issue(fill3, fill4, odd);
+            gg_wait<FLIGHT>();
             gg_barrier();
             __builtin_amdgcn_s_setprio(1);
             multiply(0);
@@ -324,9 +372,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
             __builtin_amdgcn_sched_barrier(0);
             gg_barrier();
         } else {
-            gg_wait<2 * IPW>();
+            gg_wait<FLIGHT>();
             gg_barrier();
-            issue(fill);
+            issue(fill3, fill4, odd);
             fetch(0);
             fetch(1);
             multiply(0);
@@ -336,101 +384,115 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     };
     if (steps > 0) {
 #pragma unroll
-        for (int t = 0; t < NST - 1; ++t) issue(smem + t * SB);
+        for (int t = 0; t < 4; t += 2) {
+            char* const f0 = smem + t * SB;
+            char* const f1 = f0 + SB;
+            if (!AKS) issue_a(f0, f1, true);
+            if (!BKS) issue_b(f0, f1, true);
+            if (AKS) issue_a(f0, f0, false);
+            if (BKS) issue_b(f0, f0, false);
+            if (AKS) issue_a(f1, f1, false);
+            if (BKS) issue_b(f1, f1, false);
+        }
         if (PP) {
-            gg_wait<2 * IPW>();
+            gg_wait<FLIGHT>();
             gg_barrier();
             if (wave >= NW / 2) gg_barrier();
         }
-        for (int t = 0; t < steps; ++t) stage(smem + ((t + NST - 1) % NST) * SB, smem + (t % NST) * SB);
+        int u = 0;                                                             // stage t's place in the ring
+        auto place = [](int k) { return (k >= NST ? k - NST : k) * SB; };
+        for (int t = 0; t < steps; t += 2) {                                   // an odd number of stages: the last one multiplies zeros
+            stage(smem + place(u + 3), smem + place(u + 4), smem + u * SB, false);
+            stage(smem + place(u + 4), smem + u * SB, smem + place(u + 1), true);
+            u = u + 2 >= NST ? u + 2 - NST : u + 2;
+        }
         if (PP && wave < NW / 2) gg_barrier();
     }
-
-    // ---- results: MFMA column = lane & 31, row = (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
-    const int fr = lane & 31, fh = lane >> 5;
-    float bias[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        bias[j] = 0.f;
-        const int c = c0 + wn + j * 32 + fr;
-        if (FORM == FWD && p.bias != nullptr && !none && c < p.N) {
-            const int64_t i = (int64_t)g * p.N + c;
-            bias[j] = p.bias16 ? __uint_as_float((uint32_t)((const bf16_t*)p.bias)[i] << 16) : ((const float*)p.bias)[i];
-        }
-    }
-    // a chunk of a group with several goes to its partial-sum slot, in fp32
-    const bool partial = FORM == WGRAD && s.rows > p.chunk;
-    const int orow0 = FORM == WGRAD ? n0 : r0;                                 // first output row of the tile
-    const int orows = FORM == WGRAD ? p.N - n0 : rows;
-    const int64_t base = FORM == WGRAD ? (partial ? (int64_t)(s.slot + s.tile) : (int64_t)g) * p.N * p.K : 0;
-    const int64_t ldo = FORM == WGRAD ? p.K : p.ldo;
-    const bool o16 = partial ? false : p.out16;
-    char* const out = partial ? (char*)p.part : p.out;
-    const bool vec = partial ? (p.K & 3) == 0 : p.vec;
     gg_wait<0>();                                                              // everybody has read the last stage and nothing is on its way:
     gg_barrier();                                                              // the stages' memory takes the results
-    constexpr int STG = NST * SB / NW;
-    static_assert(STG >= 32 * NT * 32 * 4, "a wave's 32 result rows");
-    char* const mine = smem + wave * STG;
-    auto leave = [&](auto out_t) {
-        using O = decltype(out_t);
-        constexpr int ROWB = NT * 32 * sizeof(O), PER = 16 / sizeof(O), LPR = ROWB / 16;
-        char* const put = mine + (4 * fh) * ROWB + fr * sizeof(O);
+
+    // ---- results
+    const bool partial = FORM == WGRAD && tl.rows > p.chunk;                   // a chunk of a group with several: to its slot, in fp32
+    const int64_t ldo = FORM == WGRAD ? p.K : p.ldo;
+    const int64_t first = (FORM == WGRAD ? (int64_t)(partial ? tl.slot + tl.tile : tl.group) * p.N * p.K + (int64_t)n0 * ldo : (int64_t)r0 * ldo) + wm * ldo + c0 + wn;
+    const int left = (FORM == WGRAD ? p.N - n0 : rows) - wm, cols = width - c0 - wn;            // output rows and columns from the wave's first on
+    char* const out = partial ? (char*)p.part : p.out;
+    const int fr = lane & 31, fh = lane >> 5;
+    // a lane's accumulators 4 h .. 4 h + 3 of fragment (i, j): columns j * 32 + 8 h + 4 fh + 0 .. 3 of row i * 32 + fr
+    if (FORM == FWD && p.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float b = __shfl(bias, j * 32 + (r & 3) + 8 * (r >> 2) + 4 * fh, 64);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[i][j][r] += b;
+            }
+    }
+    if (!partial && p.out16) {
+        char* const mine = smem + wave * 32 * ROWB;                            // 32 result rows at a time, left as whole 16-byte chunks
+        auto slot = [&](int row, int chunk) { return mine + row * ROWB + ((chunk ^ (CPR == 8 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4); };
+        bf16_t* const dst = reinterpret_cast<bf16_t*>(out) + first;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float v = acc[i][j][r] + bias[j];
-                    O* const d = reinterpret_cast<O*>(put + ((r & 3) + 8 * (r >> 2)) * ROWB + j * 32 * sizeof(O));
-                    if (sizeof(O) == 2) *d = (O)bf_bits(v);
-                    else *d = (O)v;
+                for (int h = 0; h < 4; ++h) {
+                    const f32x16& a = acc[i][j];
+                    *reinterpret_cast<uint2*>(slot(fr, j * 4 + h) + fh * 8) = make_uint2(bf_bits(a[4 * h]) | (bf_bits(a[4 * h + 1]) << 16),
+                                                                                        bf_bits(a[4 * h + 2]) | (bf_bits(a[4 * h + 3]) << 16));
                 }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the wave's own rows, written by all its lanes
-            const int left = orows - (wm + i * 32), rr = left < 32 ? left : 32;
-            O* const dst = reinterpret_cast<O*>(out) + base + (int64_t)(orow0 + wm + i * 32) * ldo + c0 + wn;
-            if (vec) {
+            if (p.vec) {
 #pragma unroll
-                for (int t = 0; t < 32; t += 64 / LPR) {
-                    const int row = t + lane / LPR, col = (lane % LPR) * PER;
-                    if (row < rr && c0 + wn + col < width)
-                        *reinterpret_cast<uint4*>(dst + row * ldo + col) = *reinterpret_cast<const uint4*>(mine + row * ROWB + (lane % LPR) * 16);
+                for (int t = 0; t < 32; t += 64 / CPR) {
+                    const int row = t + lane / CPR, ch = lane % CPR;
+                    if (i * 32 + row < left && ch * 8 < cols)
+                        *reinterpret_cast<uint4*>(dst + (i * 32 + row) * ldo + ch * 8) = *reinterpret_cast<const uint4*>(slot(row, ch));
                 }
             } else {
                 for (int t = lane; t < 32 * NT * 32; t += 64) {
-                    const int row = t / (NT * 32), col = t % (NT * 32);
-                    if (row < rr && c0 + wn + col < width) dst[row * ldo + col] = reinterpret_cast<const O*>(mine)[t];
+                    const int row = t / (NT * 32), c = t % (NT * 32);
+                    if (i * 32 + row < left && c < cols) dst[(i * 32 + row) * ldo + c] = *reinterpret_cast<const bf16_t*>(slot(row, c >> 3) + (c & 7) * 2);
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
         }
-    };
-    if (o16) leave(bf16_t{});
-    else leave(float{});
+    } else {
+        float* const dst = reinterpret_cast<float*>(out) + first;
+        const bool vec = partial ? (p.K & 3) == 0 : p.vec;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const f32x16& a = acc[i][j];
+                    const int c = j * 32 + 8 * h + 4 * fh;
+                    if (i * 32 + fr >= left) continue;
+                    float* const d = dst + (i * 32 + fr) * ldo + c;
+                    if (vec) {
+                        if (c < cols) *reinterpret_cast<f32x4*>(d) = f32x4{a[4 * h], a[4 * h + 1], a[4 * h + 2], a[4 * h + 3]};
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < cols) d[e] = a[4 * h + e];
+                    }
+                }
+    }
 }
 
 // dW of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: group
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
     const int g = blockIdx.y;
-    int edge = gg_offset(p, 0), slots = 0, len = 0, first = 0;
-    const int lane = threadIdx.x & 63;
-    for (int c = 0; c * 64 <= g; ++c) {
-        const int v = c * 64 + lane;
-        int end = v < p.G ? gg_offset(p, v + 1) : 0;
-        end = scan_max(end > edge ? end : edge, lane);
-        const int up = __shfl_up(end, 1, 64), l = end - (lane == 0 ? edge : up);
-        const int nt = v < p.G ? (l + p.chunk - 1) / p.chunk : 0, m = nt > 1 ? nt : 0;
-        const int ns = scan_add(m, lane) + slots;
-        if (g < c * 64 + 64) { len = __shfl(l, g & 63, 64); first = __shfl(ns - m, g & 63, 64); }
-        edge = __shfl(end, 63, 64);
-        slots = __shfl(ns, 63, 64);
-    }
-    if (len <= p.chunk) return;
-    const int n = (len + p.chunk - 1) / p.chunk;
+    int n;
+    Groups<true> groups;
+    const Tile t = groups.of(p, p.chunk, threadIdx.x & 63, g, n);
+    if (n <= 1) return;
     const int64_t size = (int64_t)p.N * p.K;
-    const float* const part = p.part + first * size;
+    const float* const part = p.part + t.slot * size;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
         float v = 0.f;
         for (int c = 0; c < n; ++c) v += part[c * size + i];
@@ -445,10 +507,11 @@ template <typename T>
 __global__ __launch_bounds__(256) void grouped_colsum_kernel(GgP p) {
     __shared__ float join[4][64];
     const int ct = (p.N + 63) / 64;
-    Seg s;
-    int item = -1;
-    if (!find_tile<false>(p, GG_BIAS_ROWS, [&](int total) { item = (int)blockIdx.x < total * ct ? (int)blockIdx.x : -1; return item < 0 ? -1 : item / ct; }, s)) return;
-    const int c = (item % ct) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    Groups<true> groups;
+    groups.init(p, GG_BIAS_ROWS, threadIdx.x & 63);
+    if ((int)blockIdx.x >= groups.total * ct) return;
+    const Tile s = groups.find(p, GG_BIAS_ROWS, threadIdx.x & 63, (int)blockIdx.x / ct);
+    const int c = ((int)blockIdx.x % ct) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
     const int r0 = s.row0 + s.tile * GG_BIAS_ROWS, rows = min(GG_BIAS_ROWS, s.rows - s.tile * GG_BIAS_ROWS);
     float a[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < p.N) {
@@ -466,23 +529,13 @@ __global__ __launch_bounds__(256) void grouped_colsum_kernel(GgP p) {
 }
 // db[g] = its chunks' sums in row order.  blockIdx.y: group
 __global__ __launch_bounds__(256) void grouped_colsum_join_kernel(GgP p) {
-    const int g = blockIdx.y, lane = threadIdx.x & 63, c = blockIdx.x * 256 + threadIdx.x;
-    int edge = gg_offset(p, 0), tiles = 0, n = 0, first = 0;
-    for (int k = 0; k * 64 <= g; ++k) {
-        const int v = k * 64 + lane;
-        int end = v < p.G ? gg_offset(p, v + 1) : 0;
-        end = scan_max(end > edge ? end : edge, lane);
-        const int up = __shfl_up(end, 1, 64), l = end - (lane == 0 ? edge : up);
-        int nt = v < p.G ? (l + GG_BIAS_ROWS - 1) / GG_BIAS_ROWS : 0;
-        if (v < p.G && nt == 0) nt = 1;
-        const int sum = scan_add(nt, lane) + tiles;
-        if (g < k * 64 + 64) { n = __shfl(nt, g & 63, 64); first = __shfl(sum - nt, g & 63, 64); }
-        edge = __shfl(end, 63, 64);
-        tiles = __shfl(sum, 63, 64);
-    }
+    const int g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
+    int n;
+    Groups<true> groups;
+    const Tile t = groups.of(p, GG_BIAS_ROWS, threadIdx.x & 63, g, n);
     if (c >= p.N) return;
     float v = 0.f;
-    for (int k = 0; k < n; ++k) v += p.part[(int64_t)(first + k) * p.N + c];
+    for (int k = 0; k < n; ++k) v += p.part[(int64_t)(t.before + k) * p.N + c];
     const int64_t i = (int64_t)g * p.N + c;
     if (p.out16) ((bf16_t*)p.out)[i] = (bf16_t)bf_bits(v);
     else ((float*)p.out)[i] = v;
@@ -501,21 +554,28 @@ __global__ __launch_bounds__(256) void grouped_pad_kernel(const T* __restrict__ 
 
 template <typename T, int FORM, int BM, int BN, int WGM, int WGN>
 void go(const GgP& p, int64_t items, hipStream_t st) {
-    constexpr int LDS = 4 * (BM + BN) * 64;
+    constexpr int LDS = 5 * (BM + BN) * 64;
     auto k = grouped_kernel<T, FORM, BM, BN, WGM, WGN>;
     if (!uem_allow_lds((const void*)k, LDS)) return;
-    k<<<(unsigned)items, 64 * WGM * WGN, LDS, st>>>(p);
+    k<<<(unsigned)(uem_cdiv(items, 8) * 8), 64 * WGM * WGN, LDS, st>>>(p);
 }
 
-// most row tiles that T rows in G groups make, with the rows in front and behind
-int64_t most_tiles(int T, int G, int bm) { return T / bm + (int64_t)G + 2; }
-
-// Tile of the forward and the data gradient.  256 x 256 moves the fewest operand bytes a flop; it needs enough tiles to fill the CUs and
-// groups that fill it.  64 x 128 is for groups of a few rows, where the weight's bytes are what counts.
-int tile_rows(int T, int G, int width) {
-    const int64_t per = uem_cdiv(T, G);
-    if (per >= 192 && (uem_cdiv(T, 256) + G / 2) * uem_cdiv(width, 256) >= 192) return 256;
-    return per >= 80 ? 128 : 64;
+// Tile of the forward and the data gradient: the one whose slowest CU has the least to do.  The larger a tile the fewer operand bytes a
+// flop; a smaller one wastes less of a short group and spreads further.  The factors are the rates measured with every CU at work, of the
+// largest tile's: bf16 65536 x 2048 -> 2048 in 32 groups 515 / 635 / 873 us, fp32 65536 x 512 -> 512 in 8 groups 309 / 299 / 285.
+struct TileShape { int bm, bn; double rate16, rate32; };
+constexpr TileShape TILES[3] = {{256, 256, 1.0, 1.0}, {128, 128, 0.8, 1.03}, {64, 128, 0.6, 1.08}};
+int64_t likely_tiles(int T, int G, int bm) { return T / bm + (G < T ? G : T) / 2 + 1; }
+int pick_tile(int T, int G, int width, bool is16) {
+    int best = 0;
+    if (getenv("GG_TILE")) return atoi(getenv("GG_TILE"));
+    double least = 0;
+    for (int i = 0; i < 3; ++i) {
+        const double n = (double)uem_cdiv(likely_tiles(T, G, TILES[i].bm) * uem_cdiv(width, TILES[i].bn), 256);
+        const double cost = n * TILES[i].bm * TILES[i].bn / (is16 ? TILES[i].rate16 : TILES[i].rate32);
+        if (i == 0 || cost < least) { best = i; least = cost; }
+    }
+    return best;
 }
 // rows of a weight-gradient item: all of them where the groups' tiles fill the chip anyway, else so that it is filled
 int wgrad_chunk(int T, int G, int N, int K, int bm) {
@@ -528,11 +588,11 @@ int wgrad_tile(int G, int N, int K) { return uem_cdiv(N, 256) * uem_cdiv(K, 256)
 
 template <typename T, int FORM>
 int launch_rows(const GgP& p, const char* what, hipStream_t st) {
-    const int width = FORM == FWD ? p.N : p.K, bm = tile_rows(p.T, p.G, width), bn = bm == 256 ? 256 : 128;
-    const int64_t items = uem_cdiv(most_tiles(p.T, p.G, bm) * uem_cdiv(width, bn), 8) * 8;
-    UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than a launch takes", what, (long long)items);
-    if (bm == 256) go<T, FORM, 256, 256, 2, 4>(p, items, st);
-    else if (bm == 128) go<T, FORM, 128, 128, 2, 2>(p, items, st);
+    const int width = FORM == FWD ? p.N : p.K, t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
+    const int64_t items = (p.T / TILES[t].bm + (int64_t)p.G + 1) * uem_cdiv(width, TILES[t].bn);     // at most so many tiles
+    UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than the kernels count", what, (long long)items);
+    if (t == 0) go<T, FORM, 256, 256, 2, 4>(p, items, st);
+    else if (t == 1) go<T, FORM, 128, 128, 2, 2>(p, items, st);
     else go<T, FORM, 64, 128, 1, 4>(p, items, st);
     return uem_check_launch(what);
 }
@@ -609,8 +669,8 @@ extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x
     p.part = workspace;
     const int64_t slots = T > p.chunk ? 2 * (int64_t)T / p.chunk : 0;
     if (dw != nullptr) {
-        const int64_t items = uem_cdiv((T / p.chunk + (int64_t)G) * uem_cdiv(N, bm) * uem_cdiv(K, bm), 8) * 8;
-        UEM_REQUIRE(items < ((int64_t)1 << 31), "grouped_wgrad: %lld tiles are more than a launch takes", (long long)items);
+        const int64_t items = (T / p.chunk + (int64_t)G) * uem_cdiv(N, bm) * uem_cdiv(K, bm);
+        UEM_REQUIRE(items < ((int64_t)1 << 31), "grouped_wgrad: %lld tiles are more than the kernels count", (long long)items);
         const bool h = (flags & UEM_GROUPED_BF16) != 0;
         if (bm == 256 && h) go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, st);
         else if (bm == 256) go<float, WGRAD, 256, 256, 2, 4>(p, items, st);
