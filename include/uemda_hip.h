@@ -507,7 +507,7 @@ int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld
  * not decreasing; an entry below one in front of it counts as that one, entries are clamped to [0, T].  Rows of no group: y = dx = 0.
  *   fwd    y[r]  = W_g x[r] (+ bias_g)       x [T][K], W [G][N][K], bias [G][N] or NULL, y [T][N] dense
  *   dgrad  dx[r] = W_g^T dy[r]               dx [T][K] dense
- *   wgrad  dW_g  = sum_r dy[r] x[r]^T, db_g = sum_r dy[r]; WRITTEN, zeros for an empty group; dw or db may be NULL
+ *   wgrad  dW_g  = sum_r dy[r] x[r]^T, db_g = sum_r dy[r]; WRITTEN, zeros for an empty group; db may be NULL
  * x, W, dy (and y, dx) are fp32, or bf16 with UEM_GROUPED_BF16; dW has their type, or fp32 with UEM_GROUPED_OUT_F32 (a bf16 product for an
  * fp32 master weight); bias / db are fp32, or bf16 with UEM_GROUPED_BIAS_BF16.  *_ld: row strides in ELEMENTS; rows of the operands must
  * begin on 16-byte boundaries and be followed by zeros up to the next one (whatever their stride holds beyond it) -- uem_grouped_pad copies

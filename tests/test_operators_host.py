@@ -101,7 +101,8 @@ def test_grouped_linear_refusals():
     assert lib.uem_grouped_fwd(16, 4, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1 and b"shorter" in lib.uem_last_error()
     assert lib.uem_grouped_fwd(16, 8, 16, 8, None, 16, 16, 1 << 30, 2, 8, 8, 0, None) == -1
     assert lib.uem_grouped_dgrad(16, 8, 16, 8, 16, 16, 4, 2, 8, 8, 64, None) == -1
-    assert lib.uem_grouped_wgrad(16, 8, 16, 8, 16, 16, None, 16, 4, 2, 8, 8, 0, None) == -1
+    assert lib.uem_grouped_wgrad(16, 8, 16, 8, None, 16, 16, 16, 4, 2, 8, 8, 0, None) == -1
+    assert lib.uem_grouped_wgrad(16, 8, 16, 8, 16, 16, None, 16, 1 << 20, 2, 8, 8, 0, None) == -1 and b"workspace" in lib.uem_last_error()
     assert lib.uem_grouped_pad(16, 4, 16, 8, 6, 4, 0, None) == -1
-    for T, G, K, N in ((1, 1, 1, 1), (100, 3, 5, 7), (1 << 20, 64, 2048, 2048)):
-        assert lib.uem_grouped_wgrad_workspace_floats(T, G, K, N) >= (T // 512 + G) * N
+    for T, G, K, N in ((1, 1, 1, 1), (100, 3, 5, 7), (1 << 20, 64, 2048, 2048), (1 << 20, 2, 8, 8)):
+        assert lib.uem_grouped_wgrad_workspace_floats(T, G, K, N) >= (0 if T < 1000 else N * (K + 1))

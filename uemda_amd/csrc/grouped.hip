@@ -41,12 +41,13 @@ struct GgP {
     const char* a; const char* b;                 // FWD x, W | DGRAD dy, W | WGRAD dy, x
     char* out;
     const void* bias;                             // FWD only, may be null
-    float* part;                                  // WGRAD: partial sums of groups of several row chunks
+    void* db;                                     // WGRAD: column sums of dy, may be null
+    float* part; float* part_db;                  // WGRAD: partial sums of groups of several row chunks
     const void* offsets;
     int64_t lda, ldb;                             // bytes of a row of a / of b
     int T, G, K, N, chunk;                        // K: columns of x (out of W's rows), N: columns of y;  chunk: rows of a WGRAD item
     int64_t ldo;                                  // elements of an output row
-    bool off64, bias16, out16, vec;               // 64-bit offsets; bias / output in bf16; output rows take 16-byte stores
+    bool off64, bias16, out16, vec;               // 64-bit offsets; bias or db / output in bf16; output rows take 16-byte stores
 };
 
 __device__ __forceinline__ i32x4 rsrc(const char* p, unsigned bytes) {
@@ -65,14 +66,25 @@ __device__ __forceinline__ int gg_offset(const GgP& p, int i) {
     o = o < 0 ? 0 : o;
     return (int)(o > p.T ? p.T : o);
 }
-__device__ __forceinline__ int scan_add(int v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v += u; }
+// inclusive scans over a wave by DPP: inside the rows of 16 lanes, then the rows' totals carried on (a dozen cycles a step; by LDS exchange
+// the two or three scans in front of a tile took 1 us)
+template <int CTRL, int ROWS> __device__ __forceinline__ int lane_take(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xF, false); }
+__device__ __forceinline__ int scan_add(int v) {
+    v += lane_take<0x111, 0xF>(0, v);              // row_shr 1, 2, 4, 8; lanes without a source take 0
+    v += lane_take<0x112, 0xF>(0, v);
+    v += lane_take<0x114, 0xF>(0, v);
+    v += lane_take<0x118, 0xF>(0, v);
+    v += lane_take<0x142, 0xA>(0, v);              // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+    v += lane_take<0x143, 0xC>(0, v);
     return v;
 }
-__device__ __forceinline__ int scan_max(int v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { const int u = __shfl_up(v, o, 64); if (lane >= o) v = u > v ? u : v; }
+__device__ __forceinline__ int scan_max(int v) {   // v >= 0
+    v = max(v, lane_take<0x111, 0xF>(0, v));
+    v = max(v, lane_take<0x112, 0xF>(0, v));
+    v = max(v, lane_take<0x114, 0xF>(0, v));
+    v = max(v, lane_take<0x118, 0xF>(0, v));
+    v = max(v, lane_take<0x142, 0xA>(0, v));
+    v = max(v, lane_take<0x143, 0xC>(0, v));
     return v;
 }
 __device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
@@ -88,14 +100,14 @@ struct Groups {
     __device__ __forceinline__ void load(const GgP& p, int bm, int chunk, int lane, int& edge, int& ntiles, int& nslot) {
         const int v = chunk * 64 + lane;
         int end = v < p.G ? gg_offset(p, v + 1) : 0;
-        end = scan_max(end > edge ? end : edge, lane);
+        end = scan_max(end > edge ? end : edge);
         const int up = __shfl_up(end, 1, 64);
         begin = lane == 0 ? edge : up;
         len = end - begin;
         nt = v < p.G ? (len + bm - 1) / bm : 0;
         if (ONE && v < p.G && nt == 0) nt = 1;
-        tiles = scan_add(nt, lane) + ntiles;
-        slots = ONE ? scan_add(nt > 1 ? nt : 0, lane) + nslot : 0;
+        tiles = scan_add(nt) + ntiles;
+        slots = ONE ? scan_add(nt > 1 ? nt : 0) + nslot : 0;
         loaded = chunk;
         edge = lane_value(end, 63);
         ntiles = lane_value(tiles, 63);
@@ -220,6 +232,16 @@ template <int R> struct Frag<float, true, R> {
 template <typename FA, typename FB> __device__ __forceinline__ void mma(const FA& a, const FB& b, f32x16& c, bf16_t) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
 }
+// sum of a lane's elements of a fragment (on the vector units, which the matrix cores leave idle)
+template <typename FA> __device__ __forceinline__ float sum_of(const FA& a, bf16_t) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 u = __builtin_bit_cast(u32x4, a.v);
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = __uint_as_float(u[i] << 16) + __uint_as_float(u[i] & 0xffff0000u);
+    return (s[0] + s[1]) + (s[2] + s[3]);
+}
+template <typename FA> __device__ __forceinline__ float sum_of(const FA& a, float) { return (a.v[0] + a.v[1]) + (a.v[2] + a.v[3]); }
 template <typename FA, typename FB> __device__ __forceinline__ void mma(const FA& a, const FB& b, f32x16& c, float) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
@@ -340,6 +362,10 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+    // db: the blocks of W's first columns also add up dy's columns, one fragment of them a wave
+    const bool sums = FORM == WGRAD && p.db != nullptr && c0 == 0;
+    static_assert(FORM != WGRAD || MT == WGN, "a wave for each fragment of dy's columns");
+    float colsum = 0.f;
     Frag<T, AKS, BM> fa[2][MT];
     Frag<T, BKS, BN> fb[2][NT];
     // one function with the stages being refilled and the stage being read as __restrict__ pointers: that is what tells the compiler that
@@ -357,6 +383,12 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) mma(fb[ks][j], fa[ks][i], acc[i][j], T{});
         };
+        auto add_up = [&]() {                                                  // away from the MFMAs: a branch among them costs 15 % of all blocks' time
+            if (!sums) return;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+                if (i == wave % WGN) colsum += sum_of(fa[0][i], T{}) + sum_of(fa[1][i], T{});
+        };
         // In front of stage t (PP: in stage t - 1, behind its sends) the pieces of stage t have to have landed.  Newer than the last of them
         // are, of a KS operand, three stages' pieces and, of a KC operand, those of the pair behind its own (and, t even, its partner's last).
         if (PP) {
@@ -364,6 +396,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
             fetch(1);
             issue(fill3, fill4, odd);
             gg_wait<FLIGHT>();
+            if (FORM == WGRAD) add_up();
             gg_barrier();
             __builtin_amdgcn_s_setprio(1);
             multiply(0);
@@ -380,6 +413,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
             multiply(0);
             __builtin_amdgcn_sched_barrier(0);
             multiply(1);
+            if (FORM == WGRAD) add_up();
         }
     };
     if (steps > 0) {
@@ -418,6 +452,15 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     const int left = (FORM == WGRAD ? p.N - n0 : rows) - wm, cols = width - c0 - wn;            // output rows and columns from the wave's first on
     char* const out = partial ? (char*)p.part : p.out;
     const int fr = lane & 31, fh = lane >> 5;
+    if (FORM == WGRAD) colsum += __shfl_xor(colsum, 32, 64);                    // the two halves of the wave hold other rows
+    if (sums && fh == 0) {
+        const int n = n0 + wm + (wave % WGN) * 32 + fr;
+        if (n < p.N) {
+            if (partial) p.part_db[(int64_t)(tl.slot + tl.tile) * p.N + n] = colsum;
+            else if (p.bias16) ((bf16_t*)p.db)[(int64_t)tl.group * p.N + n] = (bf16_t)bf_bits(colsum);
+            else ((float*)p.db)[(int64_t)tl.group * p.N + n] = colsum;
+        }
+    }
     // a lane's accumulators 4 h .. 4 h + 3 of fragment (i, j): columns j * 32 + 8 h + 4 fh + 0 .. 3 of row i * 32 + fr
     if (FORM == FWD && p.bias != nullptr) {
 #pragma unroll
@@ -449,7 +492,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
                 for (int t = 0; t < 32; t += 64 / CPR) {
                     const int row = t + lane / CPR, ch = lane % CPR;
                     if (i * 32 + row < left && ch * 8 < cols)
-                        *reinterpret_cast<uint4*>(dst + (i * 32 + row) * ldo + ch * 8) = *reinterpret_cast<const uint4*>(slot(row, ch));
+                        __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(slot(row, ch)), reinterpret_cast<f32x4*>(dst + (i * 32 + row) * ldo + ch * 8));
                 }
             } else {
                 for (int t = lane; t < 32 * NT * 32; t += 64) {
@@ -484,7 +527,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     }
 }
 
-// dW of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: group
+// dW and db of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: group
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
     const int g = blockIdx.y;
     int n;
@@ -493,52 +536,28 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
     if (n <= 1) return;
     const int64_t size = (int64_t)p.N * p.K;
     const float* const part = p.part + t.slot * size;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-        float v = 0.f;
-        for (int c = 0; c < n; ++c) v += part[c * size + i];
-        if (p.out16) reinterpret_cast<bf16_t*>(p.out)[g * size + i] = (bf16_t)bf_bits(v);
-        else reinterpret_cast<float*>(p.out)[g * size + i] = v;
+    if (p.vec && (size & 3) == 0) {                                            // rows of whole 16-byte stores: so is the whole of dW_g
+        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
+            f32x4 v = *reinterpret_cast<const f32x4*>(part + i);
+            for (int c = 1; c < n; ++c) v += *reinterpret_cast<const f32x4*>(part + c * size + i);
+            if (p.out16) *reinterpret_cast<uint2*>(p.out + (g * size + i) * 2) = make_uint2(bf_bits(v[0]) | (bf_bits(v[1]) << 16), bf_bits(v[2]) | (bf_bits(v[3]) << 16));
+            else *reinterpret_cast<f32x4*>(p.out + (g * size + i) * 4) = v;
+        }
+    } else {
+        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
+            float v = part[i];
+            for (int c = 1; c < n; ++c) v += part[c * size + i];
+            if (p.out16) reinterpret_cast<bf16_t*>(p.out)[g * size + i] = (bf16_t)bf_bits(v);
+            else reinterpret_cast<float*>(p.out)[g * size + i] = v;
+        }
     }
-}
-
-// db: column sums of dy per group.  Item: GG_BIAS_ROWS rows x 64 columns, four waves down the rows -> part[item's chunk][N]
-constexpr int GG_BIAS_ROWS = 512;
-template <typename T>
-__global__ __launch_bounds__(256) void grouped_colsum_kernel(GgP p) {
-    __shared__ float join[4][64];
-    const int ct = (p.N + 63) / 64;
-    Groups<true> groups;
-    groups.init(p, GG_BIAS_ROWS, threadIdx.x & 63);
-    if ((int)blockIdx.x >= groups.total * ct) return;
-    const Tile s = groups.find(p, GG_BIAS_ROWS, threadIdx.x & 63, (int)blockIdx.x / ct);
-    const int c = ((int)blockIdx.x % ct) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    const int r0 = s.row0 + s.tile * GG_BIAS_ROWS, rows = min(GG_BIAS_ROWS, s.rows - s.tile * GG_BIAS_ROWS);
-    float a[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < p.N) {
-        const char* const src = p.a + (int64_t)r0 * p.lda + (int64_t)c * sizeof(T);
-        auto at = [&](int r) { return sizeof(T) == 2 ? __uint_as_float((uint32_t)*(const bf16_t*)(src + r * p.lda) << 16) : *(const float*)(src + r * p.lda); };
-        int r = w;
-        for (; r + 12 < rows; r += 16)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) a[k] += at(r + 4 * k);
-        for (; r < rows; r += 4) a[0] += at(r);
-    }
-    join[w][threadIdx.x & 63] = (a[0] + a[1]) + (a[2] + a[3]);
-    __syncthreads();
-    if (w == 0 && c < p.N) p.part[(int64_t)(s.before + s.tile) * p.N + c] = (join[0][threadIdx.x] + join[1][threadIdx.x]) + (join[2][threadIdx.x] + join[3][threadIdx.x]);
-}
-// db[g] = its chunks' sums in row order.  blockIdx.y: group
-__global__ __launch_bounds__(256) void grouped_colsum_join_kernel(GgP p) {
-    const int g = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x;
-    int n;
-    Groups<true> groups;
-    const Tile t = groups.of(p, GG_BIAS_ROWS, threadIdx.x & 63, g, n);
-    if (c >= p.N) return;
-    float v = 0.f;
-    for (int k = 0; k < n; ++k) v += p.part[(int64_t)(t.before + k) * p.N + c];
-    const int64_t i = (int64_t)g * p.N + c;
-    if (p.out16) ((bf16_t*)p.out)[i] = (bf16_t)bf_bits(v);
-    else ((float*)p.out)[i] = v;
+    if (p.db != nullptr)
+        for (int c = blockIdx.x * 256 + threadIdx.x; c < p.N; c += gridDim.x * 256) {
+            float v = 0.f;
+            for (int k = 0; k < n; ++k) v += p.part_db[(int64_t)(t.slot + k) * p.N + c];
+            if (p.bias16) ((bf16_t*)p.db)[(int64_t)g * p.N + c] = (bf16_t)bf_bits(v);
+            else ((float*)p.db)[(int64_t)g * p.N + c] = v;
+        }
 }
 
 // dst[r][0 .. ldd) = src[r][0 .. cols), zeros behind: rows that begin on 16-byte boundaries
@@ -565,10 +584,9 @@ void go(const GgP& p, int64_t items, hipStream_t st) {
 // largest tile's: bf16 65536 x 2048 -> 2048 in 32 groups 515 / 635 / 873 us, fp32 65536 x 512 -> 512 in 8 groups 309 / 299 / 285.
 struct TileShape { int bm, bn; double rate16, rate32; };
 constexpr TileShape TILES[3] = {{256, 256, 1.0, 1.0}, {128, 128, 0.8, 1.03}, {64, 128, 0.6, 1.08}};
-int64_t likely_tiles(int T, int G, int bm) { return T / bm + (G < T ? G : T) / 2 + 1; }
+int64_t likely_tiles(int T, int G, int bm) { return uem_cdiv(T, bm) + (G < T ? G : T) / 2; }      // half a tile of each group is empty
 int pick_tile(int T, int G, int width, bool is16) {
     int best = 0;
-    if (getenv("GG_TILE")) return atoi(getenv("GG_TILE"));
     double least = 0;
     for (int i = 0; i < 3; ++i) {
         const double n = (double)uem_cdiv(likely_tiles(T, G, TILES[i].bm) * uem_cdiv(width, TILES[i].bn), 256);
@@ -577,14 +595,15 @@ int pick_tile(int T, int G, int width, bool is16) {
     }
     return best;
 }
-// rows of a weight-gradient item: all of them where the groups' tiles fill the chip anyway, else so that it is filled
-int wgrad_chunk(int T, int G, int N, int K, int bm) {
-    const int64_t tiles = uem_cdiv(N, bm) * uem_cdiv(K, bm);
-    int64_t c = uem_cdiv((int64_t)T * tiles, 256);
-    c = uem_cdiv(c < 1024 ? 1024 : c, 64) * 64;
-    return (int)(c > T ? (T < 64 ? 64 : uem_cdiv(T, 64) * 64) : c);
-}
 int wgrad_tile(int G, int N, int K) { return uem_cdiv(N, 256) * uem_cdiv(K, 256) * G >= 96 && N > 128 && K > 128 ? 256 : 128; }
+// Rows of a weight-gradient item: about what one of the 256 blocks at work (two of them a CU with 128 x 128 tiles) has to do in all, so that a
+// group with most of the rows spreads over the chip; each slot of partial sums costs N * K * 8 bytes of traffic.  Measured, us: 26215 x (2048
+// -> 512) in 7 classes, one of them with 9679 rows, 256 x 256 tiles, 512 / 1024 / 2048 / 3648 / 8192 rows: 147 / 107 / 80 / 96 / 163.
+int wgrad_chunk(int T, int G, int N, int K, int bm) {
+    const int64_t c = uem_cdiv((int64_t)T * uem_cdiv(N, bm) * uem_cdiv(K, bm), bm == 256 ? 256 : 512);
+    return (int)(uem_cdiv(c < 256 ? 256 : c < T ? c : T, 64) * 64);
+}
+int64_t wgrad_slots(int T, int chunk) { return T > chunk ? 2 * (int64_t)T / chunk : 0; }      // m > 1 chunks are of more than (m - 1) * chunk rows
 
 template <typename T, int FORM>
 int launch_rows(const GgP& p, const char* what, hipStream_t st) {
@@ -651,44 +670,32 @@ extern "C" int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w
                                       : launch_rows<float, DGRAD>(p, "grouped_dgrad", (hipStream_t)stream);
 }
 extern "C" int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N) {
-    const int bm = wgrad_tile(G, N, K), chunk = wgrad_chunk(T, G, N, K, bm);
-    // a group of m > 1 chunks has more than (m - 1) * chunk rows: at most 2 T / chunk slots in all
-    const int64_t slots = T > chunk ? 2 * (int64_t)T / chunk : 0;
-    const int64_t bias = ((int64_t)T / GG_BIAS_ROWS + G) * N;
-    return (slots * (int64_t)N * K + 3) / 4 * 4 + bias;
+    const int64_t slots = wgrad_slots(T, wgrad_chunk(T, G, N, K, wgrad_tile(G, N, K)));
+    return (slots * (int64_t)N * K + 3) / 4 * 4 + slots * N;
 }
 extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x_ld, void* dw, void* db, float* workspace, const void* offsets, int T,
                                  int G, int K, int N, int flags, void* stream) {
-    const int rc = check(dy, x, dw ? dw : db, offsets, T, G, K, N, dy_ld, x_ld, flags, "grouped_wgrad");
+    const int rc = check(dy, x, dw, offsets, T, G, K, N, dy_ld, x_ld, flags, "grouped_wgrad");
     if (rc != UEM_OK) return rc;
-    UEM_REQUIRE(dy_ld >= N && x_ld >= K && workspace && ((uintptr_t)workspace & 15) == 0, "grouped_wgrad: bad row strides or workspace");
+    UEM_REQUIRE(dy_ld >= N && x_ld >= K, "grouped_wgrad: row strides shorter than the rows");
     hipStream_t st = (hipStream_t)stream;
     GgP p = params(dy, dy_ld, x, x_ld, dw, K, offsets, T, G, K, N, flags);
     const int bm = wgrad_tile(G, N, K);
     p.chunk = wgrad_chunk(T, G, N, K, bm);
+    const int64_t slots = wgrad_slots(T, p.chunk), items = (T / p.chunk + (int64_t)G) * uem_cdiv(N, bm) * uem_cdiv(K, bm);
+    UEM_REQUIRE(slots == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "grouped_wgrad: no workspace, or not on a 16-byte boundary");
+    UEM_REQUIRE(items < ((int64_t)1 << 31), "grouped_wgrad: %lld tiles are more than the kernels count", (long long)items);
+    p.db = db;
     p.part = workspace;
-    const int64_t slots = T > p.chunk ? 2 * (int64_t)T / p.chunk : 0;
-    if (dw != nullptr) {
-        const int64_t items = (T / p.chunk + (int64_t)G) * uem_cdiv(N, bm) * uem_cdiv(K, bm);
-        UEM_REQUIRE(items < ((int64_t)1 << 31), "grouped_wgrad: %lld tiles are more than the kernels count", (long long)items);
-        const bool h = (flags & UEM_GROUPED_BF16) != 0;
-        if (bm == 256 && h) go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, st);
-        else if (bm == 256) go<float, WGRAD, 256, 256, 2, 4>(p, items, st);
-        else if (h) go<bf16_t, WGRAD, 128, 128, 2, 2>(p, items, st);
-        else go<float, WGRAD, 128, 128, 2, 2>(p, items, st);
-        if (slots > 0) {
-            int64_t nb = uem_cdiv((int64_t)N * K, 256 * 4);
-            grouped_join_kernel<<<dim3((unsigned)(nb < 1024 ? nb : 1024), (unsigned)G), 256, 0, st>>>(p);
-        }
-    }
-    if (db != nullptr) {
-        p.out = (char*)db;
-        p.out16 = (flags & UEM_GROUPED_BIAS_BF16) != 0;
-        p.part = workspace + (slots * (int64_t)N * K + 3) / 4 * 4;
-        const int64_t items = (T / GG_BIAS_ROWS + (int64_t)G) * uem_cdiv(N, 64);
-        if (flags & UEM_GROUPED_BF16) grouped_colsum_kernel<bf16_t><<<(unsigned)items, 256, 0, st>>>(p);
-        else grouped_colsum_kernel<float><<<(unsigned)items, 256, 0, st>>>(p);
-        grouped_colsum_join_kernel<<<dim3((unsigned)uem_cdiv(N, 256), (unsigned)G), 256, 0, st>>>(p);
+    p.part_db = workspace + (slots * (int64_t)N * K + 3) / 4 * 4;
+    const bool h = (flags & UEM_GROUPED_BF16) != 0;
+    if (bm == 256 && h) go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, st);
+    else if (bm == 256) go<float, WGRAD, 256, 256, 2, 4>(p, items, st);
+    else if (h) go<bf16_t, WGRAD, 128, 128, 2, 2>(p, items, st);
+    else go<float, WGRAD, 128, 128, 2, 2>(p, items, st);
+    if (slots > 0) {
+        const int64_t nb = uem_cdiv((int64_t)N * K, 1024);
+        grouped_join_kernel<<<dim3((unsigned)(nb < 512 ? nb : 512), (unsigned)G), 256, 0, st>>>(p);
     }
     return uem_check_launch("grouped_wgrad");
 }

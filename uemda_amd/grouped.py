@@ -73,10 +73,10 @@ class _GroupedLinearFn(Function):
         need_x, need_w, _, need_b = ctx.needs_input_grad
         dev = xo.device
         dx = torch.empty((T, K), device=dev, dtype=xo.dtype) if need_x else None
-        dw = torch.empty((G, N, K), device=dev, dtype=w_dtype) if need_w else None
+        dw = torch.empty((G, N, K), device=dev, dtype=w_dtype) if need_w or need_b else None      # db falls off dw's products
         db = torch.empty((G, N), device=dev, dtype=b_dtype) if need_b else None
         if T == 0:
-            return dx, None if dw is None else dw.zero_(), None, None if db is None else db.zero_()
+            return dx, dw.zero_() if need_w else None, None, None if db is None else db.zero_()
         flags = _flags(xo, offsets)
         with ops.on_device_of(xo):
             dyo, dy_ld = _operand(dy)
@@ -88,7 +88,7 @@ class _GroupedLinearFn(Function):
                 call("uem_grouped_wgrad", ptr(dyo), dy_ld, ptr(xo), xo.stride(0) if T > 1 else xo.shape[1], ptr(dw), ptr(db), ptr(ws), ptr(offsets),
                      T, G, K, N, flags | (_lib.GROUPED_OUT_F32 if w_dtype == torch.float32 else 0)
                      | (_lib.GROUPED_BIAS_BF16 if b_dtype == torch.bfloat16 else 0), stream())
-        return dx, dw, None, db
+        return dx, dw if need_w else None, None, db
 
 
 def grouped_linear(x, weight, offsets, bias=None):
