@@ -174,8 +174,6 @@ UEM_NORM_BLOCKS = 1024
 UEM_MULTI_BLOCKS = 8192
 CONV_IN_AFFINE, CONV_IN_RELU, CONV_ACCUMULATE, CONV_TRANSPOSED = 1, 2, 4, 8
 CONV_PREC_BF16 = 32
-LN_BF16, LN_PARAM_BF16 = 1, 2
-GROUPED_BF16, GROUPED_OUT_F32, GROUPED_BIAS_BF16, GROUPED_OFFSETS_64 = 1, 2, 4, 8
 PREP_TRANSPOSE, PREP_WINO2, PREP_WINO2_T, PREP_WINO4, PREP_WINO4_T, PREP_STEM_PACK, PREP_TRANSPOSE_BF16 = range(7)
 
 
@@ -210,6 +208,23 @@ def load():
         fn.restype = _RESTYPE.get(name, c_int)
     _lib = lib
     return lib
+
+
+_host = None
+
+
+def host():
+    """The extension with the host side of norm / grouped / optim's operators, its entry points bound to the loaded library's."""
+    global _host
+    if _host is None:
+        lib = load()
+        try:
+            from . import _host as ext
+        except ImportError as e:
+            raise UemError(f"uemda_amd/_host.so cannot be imported ({e}): run `python -c 'import __graft_entry__ as g; g.build()'`") from e
+        ext.bind(UemError, {name: ctypes.cast(getattr(lib, name), c_void_p).value for name in ext.names()})
+        _host = ext
+    return _host
 
 
 ERR_UNSUPPORTED = -2          # UEM_ERR_UNSUPPORTED: the entry point does not take this configuration and launched nothing

@@ -256,6 +256,24 @@ __device__ __forceinline__ void gg_barrier() {
     asm volatile("" ::: "memory");
 }
 
+// rows of no group, shared out over the grid: zeros
+template <int NTH>
+__device__ __forceinline__ void zero_rows(const GgP& p, const Groups<false>& groups, int width) {
+    const int head = groups.first, zeros = head + p.T - groups.last;
+    for (int z = blockIdx.x; z < zeros; z += gridDim.x) {
+        const int64_t at = (int64_t)(z < head ? z : groups.last + z - head) * p.ldo;
+        if (p.vec) {
+            const int n = p.out16 ? 8 : 4;
+            for (int c = threadIdx.x * n; c < width; c += NTH * n) *reinterpret_cast<uint4*>(p.out + (at + c) * (p.out16 ? 2 : 4)) = make_uint4(0, 0, 0, 0);
+        } else {
+            for (int c = threadIdx.x; c < width; c += NTH)
+                if (p.out16) reinterpret_cast<bf16_t*>(p.out)[at + c] = 0;
+                else reinterpret_cast<float*>(p.out)[at + c] = 0.f;
+        }
+    }
+}
+template <int NTH> __device__ __forceinline__ void zero_rows(const GgP&, const Groups<true>&, int) {}
+
 // One tile a block.  Five stages: while stage t is computed on, a KS operand's pieces of stage t + 4 leave, a KC operand's of stages t + 3 and
 // t + 4 together if t is odd -- the two halves of every 128-byte line one after the other, or the line travels from L2 twice (65536 x 2048 ->
 // 2048 in 32 groups, forward: 545 us stage by stage, 515 in pairs; KS operands in pairs lose: weight gradient 488 against 529).
@@ -279,21 +297,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     Groups<FORM == WGRAD> groups;
     groups.init(p, bm, lane);
 
-    // ---- rows of no group: zeros
-    if (FORM != WGRAD) {
-        const int head = groups.first, zeros = head + p.T - groups.last;
-        for (int z = blockIdx.x; z < zeros; z += gridDim.x) {
-            const int64_t at = (int64_t)(z < head ? z : groups.last + z - head) * p.ldo;
-            if (p.vec) {
-                const int n = p.out16 ? 8 : 4;
-                for (int c = tid * n; c < width; c += 64 * NW * n) *reinterpret_cast<uint4*>(p.out + (at + c) * (p.out16 ? 2 : 4)) = make_uint4(0, 0, 0, 0);
-            } else {
-                for (int c = tid; c < width; c += 64 * NW)
-                    if (p.out16) reinterpret_cast<bf16_t*>(p.out)[at + c] = 0;
-                    else reinterpret_cast<float*>(p.out)[at + c] = 0.f;
-            }
-        }
-    }
+    if (FORM != WGRAD) zero_rows<64 * NW>(p, groups, width);
     const int item = xcd_item(groups.total * ct * rt);
     if (item < 0) return;
 
@@ -527,6 +531,62 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     }
 }
 
+// The forward of a few rows: the weights' bytes are all there is, and the latency of reaching them.  A tile is 32 rows x 32 columns, its
+// reduction shared out over sixteen waves that load their fragments straight into registers -- at 2048 channels a wave has all of its 8 KB
+// of W on the way at once -- and are joined through LDS in wave order.  Nine rows in six groups, 2048 -> 512: 13.5 -> 7.2 us.
+template <typename T>
+__global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
+    constexpr int ES = sizeof(T), PER = 16 / ES, NW = 16, LD = 36, DEEP = 8;   // LD: floats of a staged row, off the bank period
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* const red = reinterpret_cast<float*>(smem);
+    const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Groups<false> groups;
+    groups.init(p, 32, lane);
+    zero_rows<1024>(p, groups, p.N);
+    const int ct = (p.N + 31) / 32, item = xcd_item(groups.total * ct);
+    if (item < 0) return;
+    const Tile tl = groups.find(p, 32, lane, item / ct);
+    const int c0 = (item % ct) * 32, r0 = tl.row0 + tl.tile * 32, rows = min(32, tl.rows - tl.tile * 32);
+    // lanes of rows and columns past the end read the last one again; their results are not stored
+    const char* const px = p.a + (int64_t)(r0 + min(fr, rows - 1)) * p.lda;
+    const char* const pw = p.b + ((int64_t)tl.group * p.N + min(c0 + fr, p.N - 1)) * p.ldb;
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+    const int steps = (p.K + 2 * PER - 1) / (2 * PER);                         // a lane's 16 bytes are chunk 2 * step + fh
+    for (int s0 = wave; s0 < steps; s0 += NW * DEEP) {
+        Frag<T, false, 32> x[DEEP], w[DEEP];
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) {
+            const int chunk = 2 * (s0 + k * NW) + fh;
+            const bool on = chunk * PER < p.K;
+            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+            const f32x4 vx = on ? *reinterpret_cast<const f32x4*>(px + chunk * 16) : zero, vw = on ? *reinterpret_cast<const f32x4*>(pw + chunk * 16) : zero;
+            x[k].v = __builtin_bit_cast(decltype(x[k].v), vx);
+            w[k].v = __builtin_bit_cast(decltype(w[k].v), vw);
+        }
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k) mma(w[k], x[k], acc, T{});
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h)                                                // rows of the result: columns 8 h + 4 fh + 0 .. 3 of feature row fr
+        *reinterpret_cast<f32x4*>(red + (wave * 32 + fr) * LD + 8 * h + 4 * fh) = f32x4{acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
+    __syncthreads();
+    const int m = threadIdx.x >> 5, n = threadIdx.x & 31;
+    if (m >= rows || c0 + n >= p.N) return;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) v += red[(w * 32 + m) * LD + n];
+    if (p.bias != nullptr) {
+        const int64_t i = (int64_t)tl.group * p.N + c0 + n;
+        v += p.bias16 ? __uint_as_float((uint32_t)((const bf16_t*)p.bias)[i] << 16) : ((const float*)p.bias)[i];
+    }
+    const int64_t at = (int64_t)(r0 + m) * p.ldo + c0 + n;
+    if (p.out16) reinterpret_cast<bf16_t*>(p.out)[at] = (bf16_t)bf_bits(v);
+    else reinterpret_cast<float*>(p.out)[at] = v;
+}
+
 // dW and db of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: group
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
     const int g = blockIdx.y;
@@ -605,8 +665,18 @@ int wgrad_chunk(int T, int G, int N, int K, int bm) {
 }
 int64_t wgrad_slots(int T, int chunk) { return T > chunk ? 2 * (int64_t)T / chunk : 0; }      // m > 1 chunks are of more than (m - 1) * chunk rows
 
+// 32 x 32 tiles of sixteen waves: while they are no more than the CUs and rows are long enough to share out.  Measured, us, tiles / these:
+// 6 groups 2048 -> 512 with 9, 256, 512 rows 13.5 / 7.2, 13.6 / 10.1, 14.1 / 17.8; 64 groups 1024 -> 1024 with 9, 64 rows (2048 tiles) 8.3 /
+// 10.5, 21.0 / 31.5; 8 groups 64 -> 64 3.8 / 4.5.
+bool few_rows(const GgP& p, int es) { return likely_tiles(p.T, p.G, 32) * uem_cdiv(p.N, 32) <= 256 && p.K * es >= 512; }
 template <typename T, int FORM>
 int launch_rows(const GgP& p, const char* what, hipStream_t st) {
+    if (FORM == FWD && few_rows(p, sizeof(T))) {
+        const int64_t items = (p.T / 32 + (int64_t)p.G) * uem_cdiv(p.N, 32);
+        constexpr int LDS = 16 * 32 * 36 * 4;
+        if (uem_allow_lds((const void*)grouped_few_kernel<T>, LDS)) grouped_few_kernel<T><<<(unsigned)(uem_cdiv(items, 8) * 8), 1024, LDS, st>>>(p);
+        return uem_check_launch(what);
+    }
     const int width = FORM == FWD ? p.N : p.K, t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
     const int64_t items = (p.T / TILES[t].bm + (int64_t)p.G + 1) * uem_cdiv(width, TILES[t].bn);     // at most so many tiles
     UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than the kernels count", what, (long long)items);

@@ -435,31 +435,6 @@ def need_gpu(*tensors):
                            "(there is no CPU / PyTorch fallback)")
 
 
-class _HereAlready:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE_ALREADY = _HereAlready()
-
-
-def on_device_of(t):
-    """context in which t's device is the current one (launches go to the current device's current stream)"""
-    if t.device.index == torch.cuda.current_device():
-        return _HERE_ALREADY
-    return torch.cuda.device(t.device)
-
-
-def no_second_derivative(what):
-    """first line of a backward whose kernels autograd cannot see through: with create_graph=True it would return gradients that silently
-    count as constants"""
-    if torch.is_grad_enabled():
-        raise UemError(f"{what}: a gradient of the gradient is not offered (create_graph=True)")
-
-
 def _f32c(t, what):
     if t.dtype != torch.float32 or not t.is_contiguous():
         raise UemError(f"{what}: expected a contiguous float32 tensor, got {t.dtype} strides={t.stride()}")

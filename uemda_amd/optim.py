@@ -1,7 +1,5 @@
 """clip_grad_norm_ + SGD(momentum, weight_decay) fused over the model's flat arenas
 (reference tools/train_ssl_uem.py:169-170,228-232: torch.optim.SGD + clip_grad.clip_grad_norm_(32))."""
-from array import array
-
 import torch
 
 from . import _lib, ops
@@ -10,8 +8,8 @@ from .ops import UemError, call, ptr, stream
 
 def _arena_of(params):
     """the model whose flat arenas hold all of `params`, or None"""
-    owners = {id(getattr(p, "_uem_owner", None)) for p in params}
-    return getattr(params[0], "_uem_owner", None) if len(owners) == 1 else None
+    owner = getattr(params[0], "_uem_owner", None) if params else None
+    return owner if owner is not None and all(getattr(p, "_uem_owner", None) is owner for p in params) else None
 
 
 def grad_norm(model):
@@ -30,68 +28,12 @@ def _norm_kind(norm_type, what):
     return kind
 
 
-def _dense(t):
-    """does t cover its elements' memory without gaps or overlaps, in whatever order of dimensions?"""
-    expect = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
-        if stride != expect:
-            return False
-        expect *= size
-    return True
-
-
-_KINDS = {torch.float32: 0, torch.bfloat16: 1}
-
-
-def _multi(name, tensors, what, kind, *more):
-    """uem_multi_norm / uem_multi_clip over a list of dense tensors -> the norm, a 0-dim device tensor"""
-    dev = tensors[0].get_device()
-    ptrs, numels, kinds = [], [], []
-    for t in tensors:                  # (a list of a few hundred: every attribute looked up here costs 10-20 us a call)
-        k = _KINDS.get(t.dtype)
-        if k is None:
-            raise UemError(f"{what}: gradients must be float32 or bfloat16 tensors, got {t.dtype}")
-        if t.get_device() != dev or dev < 0:
-            raise UemError(f"{what}: all gradients must be on one MI355X device, got {tensors[0].device} and {t.device} "
-                           "(there is no CPU / PyTorch fallback)")
-        kinds.append(k)
-        numels.append(t.numel())
-        ptrs.append(t.data_ptr())
-    n = len(tensors)
-    ptrs, numels = array("Q", ptrs), array("q", numels)
-    partial = torch.empty(_lib.UEM_MULTI_BLOCKS + 2 * n, device=tensors[0].device, dtype=torch.float64)
-    norm = torch.empty((), device=tensors[0].device, dtype=torch.float32)
-    with ops.on_device_of(norm):
-        call(name, ptrs.buffer_info()[0], numels.buffer_info()[0], bytes(kinds), n, kind, ptr(partial), ptr(norm), *more, stream())
-    return norm
-
-
-def _strided(t, what):
-    if t.layout != torch.strided:
-        raise UemError(f"{what}: gradients must be dense tensors, got {t.layout}")
-
-
-def _listed(tensors, what):
-    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    for t in tensors:
-        if not isinstance(t, torch.Tensor):
-            raise UemError(f"{what}: expected tensors, got {type(t).__name__}")
-    return tensors
-
-
 def get_total_norm(tensors, norm_type=2.0):
     """The norm over all elements of all `tensors` (a tensor or an iterable; fp32 and bf16 may be mixed), as a 0-dim fp32 device tensor:
     torch.nn.utils.get_total_norm for norm_type 2 or inf.  Squares are summed in 64 bits, in a fixed order; no value is read on the host."""
     what = "get_total_norm"
-    kind = _norm_kind(norm_type, what)
-    tensors = _listed(tensors, what)
-    if not tensors:
-        return torch.tensor(0.0)
-    for i, t in enumerate(tensors):
-        _strided(t, what)
-        if not t.is_contiguous() and not _dense(t):
-            tensors[i] = t.detach().contiguous()
-    return _multi("uem_multi_norm", tensors, what, kind)
+    norm = _lib.host().multi_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), what, _norm_kind(norm_type, what), False, None)
+    return torch.tensor(0.0) if norm is None else norm
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2):
@@ -102,10 +44,15 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2):
     model arena, or a model together with other modules, fp32 and bf16 mixed -- is clipped tensor by tensor in two passes over the list;
     parameters without a gradient are skipped, gradients that share memory are refused."""
     what = "clip_grad_norm_"
-    params = _listed(parameters, what)
-    model = _arena_of(params) if params else None
+    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    model = _arena_of(params)
     if model is None:
-        return _clip_tensors([g for g in [p.grad for p in params] if g is not None], params, float(max_norm), _norm_kind(norm_type, what))
+        kind, max_norm = _norm_kind(norm_type, what), float(max_norm)
+        if not max_norm >= 0.0:
+            raise UemError(f"{what}: max_norm must not be negative, got {max_norm}")
+        ops.grad_join()            # gradients of arena parameters among them may still be on the side / second stream
+        norm = _lib.host().multi_norm(params, what, kind, True, max_norm)
+        return torch.zeros((), device=params[0].device if params else "cpu") if norm is None else norm
     if norm_type != 2:
         raise UemError("clip_grad_norm_: only the L2 norm is implemented for a model's flat arena")
     arena, garena, n = model.flat_parameters()
@@ -114,29 +61,6 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2):
     coef = torch.clamp(float(max_norm) / (norm + 1e-6), max=1.0)      # one scalar
     call("uem_scale_by_scalar", ptr(garena), None, n, ptr(coef), stream())
     return norm[0]
-
-
-@torch.no_grad()
-def _clip_tensors(grads, params, max_norm, kind):
-    what = "clip_grad_norm_"
-    if not max_norm >= 0.0:
-        raise UemError(f"{what}: max_norm must not be negative, got {max_norm}")
-    if not grads:
-        return torch.zeros((), device=params[0].device if params else "cpu")
-    ops.grad_join()                # gradients of arena parameters may still be on the side / second stream
-    copies = []
-    for i, g in enumerate(grads):
-        _strided(g, what)
-        if not g.is_contiguous() and not _dense(g):
-            if any(st == 0 and sz > 1 for st, sz in zip(g.stride(), g.shape)):
-                raise UemError(f"{what}: a gradient of shape {tuple(g.shape)}, strides {g.stride()} repeats its elements: it cannot be scaled in place")
-            grads[i] = g.contiguous()
-            copies.append((g, grads[i]))
-    norm = _multi("uem_multi_clip", grads, what, kind, max_norm)
-    torch.autograd.graph.increment_version(grads)      # written through raw pointers: autograd must see the change all the same
-    for g, c in copies:            # gradients with gaps between their elements were scaled in a dense copy
-        g.copy_(c)
-    return norm
 
 
 class FusedSGD(torch.optim.Optimizer):
