@@ -620,14 +620,19 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
         }
 }
 
-// dst[r][0 .. ldd) = src[r][0 .. cols), zeros behind: rows that begin on 16-byte boundaries
+// dst[r][0 .. 8 cpr) = src[r][0 .. cols), zeros behind: rows that begin on 16-byte boundaries (cpr chunks of 16 bytes each, one a thread)
 template <typename T>
-__global__ __launch_bounds__(256) void grouped_pad_kernel(const T* __restrict__ src, int64_t lds, T* __restrict__ dst, int ldd, int cols, int64_t rows) {
-    const int64_t n = rows * ldd;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / ldd;
-        const int c = (int)(i - r * ldd);
-        dst[i] = c < cols ? src[r * lds + c] : (T)0;
+__global__ __launch_bounds__(256) void grouped_pad_kernel(const T* __restrict__ src, int64_t lds, T* __restrict__ dst, int cpr, int cols, int64_t chunks) {
+    constexpr int PER = 16 / sizeof(T);
+    struct __attribute__((aligned(16))) Chunk { T e[PER]; };
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < chunks; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = chunks < ((int64_t)1 << 31) ? (int64_t)((uint32_t)i / (uint32_t)cpr) : i / cpr;
+        const int c = (int)(i - r * cpr) * PER;
+        const T* const p = src + r * lds + c;
+        Chunk v;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) v.e[k] = c + k < cols ? p[k] : (T)0;
+        reinterpret_cast<Chunk*>(dst)[i] = v;
     }
 }
 
@@ -713,11 +718,14 @@ GgP params(const void* a, int lda, const void* b, int ldb, void* out, int ldo, c
 }  // namespace
 
 extern "C" int uem_grouped_pad(const void* src, int64_t src_ld, void* dst, int dst_ld, int cols, int64_t rows, int flags, void* stream) {
-    UEM_REQUIRE(src && dst && rows > 0 && cols > 0 && dst_ld >= cols && src_ld >= cols, "grouped_pad: bad arguments");
-    const int grid = uem_stream_grid(rows * dst_ld, 256);
+    const int per = (flags & UEM_GROUPED_BF16) ? 8 : 4;
+    UEM_REQUIRE(src && dst && rows > 0 && cols > 0 && dst_ld >= cols && dst_ld % per == 0 && src_ld >= cols && ((uintptr_t)dst & 15) == 0,
+                "grouped_pad: bad arguments (the copy's rows begin on 16-byte boundaries)");
+    const int64_t chunks = rows * (dst_ld / per);
+    const int grid = uem_stream_grid(chunks, 256);
     hipStream_t st = (hipStream_t)stream;
-    if (flags & UEM_GROUPED_BF16) grouped_pad_kernel<bf16_t><<<grid, 256, 0, st>>>((const bf16_t*)src, src_ld, (bf16_t*)dst, dst_ld, cols, rows);
-    else grouped_pad_kernel<float><<<grid, 256, 0, st>>>((const float*)src, src_ld, (float*)dst, dst_ld, cols, rows);
+    if (per == 8) grouped_pad_kernel<bf16_t><<<grid, 256, 0, st>>>((const bf16_t*)src, src_ld, (bf16_t*)dst, dst_ld / per, cols, chunks);
+    else grouped_pad_kernel<float><<<grid, 256, 0, st>>>((const float*)src, src_ld, (float*)dst, dst_ld / per, cols, chunks);
     return uem_check_launch("grouped_pad");
 }
 extern "C" int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void* bias, void* y, const void* offsets, int T, int G, int K,
