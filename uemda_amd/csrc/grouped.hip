@@ -477,35 +477,33 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
             }
     }
     if (!partial && p.out16) {
-        char* const mine = smem + wave * 32 * ROWB;                            // 32 result rows at a time, left as whole 16-byte chunks
+        char* const mine = smem + wave * MT * 32 * ROWB;                       // the wave's result rows, to leave as whole 16-byte chunks
+        static_assert(NW * MT * 32 * ROWB <= NST * SB, "the results in the stages' memory");
         auto slot = [&](int row, int chunk) { return mine + row * ROWB + ((chunk ^ (CPR == 8 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4); };
         bf16_t* const dst = reinterpret_cast<bf16_t*>(out) + first;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     const f32x16& a = acc[i][j];
-                    *reinterpret_cast<uint2*>(slot(fr, j * 4 + h) + fh * 8) = make_uint2(bf_bits(a[4 * h]) | (bf_bits(a[4 * h + 1]) << 16),
-                                                                                        bf_bits(a[4 * h + 2]) | (bf_bits(a[4 * h + 3]) << 16));
+                    *reinterpret_cast<uint2*>(slot(i * 32 + fr, j * 4 + h) + fh * 8) = make_uint2(bf_bits(a[4 * h]) | (bf_bits(a[4 * h + 1]) << 16),
+                                                                                                 bf_bits(a[4 * h + 2]) | (bf_bits(a[4 * h + 3]) << 16));
                 }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // the wave's own rows, written by all its lanes
-            if (p.vec) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                     // the wave's own rows, written by all its lanes
+        if (p.vec) {                                                           // streamed: nothing of this launch reads them (12 % of short reductions' time)
 #pragma unroll
-                for (int t = 0; t < 32; t += 64 / CPR) {
-                    const int row = t + lane / CPR, ch = lane % CPR;
-                    if (i * 32 + row < left && ch * 8 < cols)
-                        __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(slot(row, ch)), reinterpret_cast<f32x4*>(dst + (i * 32 + row) * ldo + ch * 8));
-                }
-            } else {
-                for (int t = lane; t < 32 * NT * 32; t += 64) {
-                    const int row = t / (NT * 32), c = t % (NT * 32);
-                    if (i * 32 + row < left && c < cols) dst[(i * 32 + row) * ldo + c] = *reinterpret_cast<const bf16_t*>(slot(row, c >> 3) + (c & 7) * 2);
-                }
+            for (int t = 0; t < MT * 32; t += 64 / CPR) {
+                const int row = t + lane / CPR, ch = lane % CPR;
+                if (row < left && ch * 8 < cols)
+                    __builtin_nontemporal_store(*reinterpret_cast<const f32x4*>(slot(row, ch)), reinterpret_cast<f32x4*>(dst + row * ldo + ch * 8));
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
+        } else {
+            for (int t = lane; t < MT * 32 * NT * 32; t += 64) {
+                const int row = t / (NT * 32), c = t % (NT * 32);
+                if (row < left && c < cols) dst[row * ldo + c] = *reinterpret_cast<const bf16_t*>(slot(row, c >> 3) + (c & 7) * 2);
+            }
         }
     } else {
         float* const dst = reinterpret_cast<float*>(out) + first;

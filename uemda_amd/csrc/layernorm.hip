@@ -51,6 +51,7 @@ struct LnP {
     void* y;                      // forward: y; backward: dx
     float* mean; float* rstd;     // [rows] each; forward may be null (nothing to save)
     float* part;                  // backward: [blocks][2][C] or null (no parameter gradients)
+    void* dgamma; void* dbeta;    // backward: the gradients themselves, written by a launch of one block (either may be null)
     int64_t rows, x_ld, dy_ld;
     int C, period;
     float eps;
@@ -206,6 +207,22 @@ __global__ __launch_bounds__(256) void layernorm_fwd_kernel(const LnP p) {
 // U rows of a team are in flight together: their loads are issued before the first reduction
 template <typename T, int LPR, int NV, int MODE, int U>
 __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
+    // where column c's sums of this block go
+    auto leave = [&](int c, float w, float b) {
+        if (gridDim.x > 1) {
+            float* const out = p.part + (int64_t)blockIdx.x * 2 * p.C;
+            out[c] = w;
+            out[p.C + c] = b;
+            return;
+        }
+        auto one = [&](void* to, float v) {
+            if (to == nullptr) return;
+            if (p.p16) Vec<bf16_t>::store1((bf16_t*)to + c, v);
+            else ((float*)to)[c] = v;
+        };
+        one(p.dgamma, w);
+        one(p.dbeta, b);
+    };
     using R = Row<T, LPR, NV, MODE>;
     constexpr int W = R::W, TEAMS = 256 / LPR, CAP = LPR > 64 ? 1 : LPR * NV * W;
     __shared__ float red[16 * U];
@@ -264,14 +281,13 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
         }
     }
     if (p.part == nullptr) return;
-    float* const out = p.part + (int64_t)blockIdx.x * 2 * p.C;
     if (LPR > 64) {                                                            // one team a block: straight out
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 const int c = R::col(i, lane, shift) + e;
-                if (c >= 0 && c < p.C) { out[c] = aw[i][e]; out[p.C + c] = ab[i][e]; }
+                if (c >= 0 && c < p.C) leave(c, aw[i][e], ab[i][e]);
             }
         return;
     }
@@ -296,7 +312,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
         }
         __syncthreads();
     }
-    for (int c = threadIdx.x; c < p.C; c += 256) { out[c] = join[0][c]; out[p.C + c] = join[1][c]; }
+    for (int c = threadIdx.x; c < p.C; c += 256) leave(c, join[0][c], join[1][c]);
 }
 
 // Any row length, any alignment: a block per row that reads the row again for each sum (rows beyond the register kernels' 8192
@@ -415,7 +431,7 @@ int go(const LnP& p, bool bwd, hipStream_t st) {
     if (MODE == 1) nb = uem_cdiv(nb, 8) * 8;                                   // teams % period == 0 (period <= 8)
     if (bwd) layernorm_bwd_kernel<T, LPR, NV, MODE, UB><<<(int)nb, 256, 0, st>>>(p);
     else layernorm_fwd_kernel<T, LPR, NV, MODE><<<(int)nb, 256, 0, st>>>(p);
-    return (int)nb;
+    return bwd && nb == 1 ? 0 : (int)nb;                                       // 0: no partial sums left
 }
 
 template <typename T>
@@ -490,9 +506,10 @@ extern "C" int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, in
     LnP p{};
     p.x = x; p.dy = dy; p.gamma = gamma; p.y = dx; p.mean = const_cast<float*>(mean); p.rstd = const_cast<float*>(rstd);
     p.part = dgamma || dbeta ? workspace : nullptr;
+    p.dgamma = dgamma; p.dbeta = dbeta;
     p.rows = rows; p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = C; p.p16 = (flags & UEM_LN_PARAM_BF16) != 0;
     hipStream_t st = (hipStream_t)stream;
     const int nb = (flags & UEM_LN_BF16) ? run<bf16_t>(p, true, st) : run<float>(p, true, st);
-    if (p.part) layernorm_params_kernel<<<(int)uem_cdiv(2 * (int64_t)C, 16), 1024, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
+    if (p.part && nb > 0) layernorm_params_kernel<<<(int)uem_cdiv(2 * (int64_t)C, 16), 1024, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
     return uem_check_launch("layernorm_bwd");
 }
