@@ -195,6 +195,61 @@ def test_a_second_derivative_is_refused():
         torch.autograd.grad(y.sum(), x, create_graph=True)
 
 
+def test_a_capture_beside_an_eager_graph_of_the_same_leaves_is_refused():
+    """(the engine would end the process) -- and is fine once that graph is gone"""
+    from uemda_amd import UemError
+    from uemda_amd.grouped import grouped_linear
+    from uemda_amd.norm import layer_norm
+    x = torch.randn(6, 16, device="cuda", requires_grad=True)
+    w = torch.randn(2, 8, 16, device="cuda", requires_grad=True)
+    off = torch.tensor([0, 2, 6], device="cuda")
+    dy, dz = torch.randn(6, 16, device="cuda"), torch.randn(6, 8, device="cuda")
+    want = torch.autograd.grad(layer_norm(x), x, dy)[0], torch.autograd.grad(grouped_linear(x, w, off), (x, w), dz)
+    held = layer_norm(x), grouped_linear(x, w, off)
+    for f in (lambda: layer_norm(x), lambda: grouped_linear(x.detach(), w, off)):
+        with pytest.raises(UemError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                f()
+        torch.cuda.synchronize()
+    with torch.no_grad():                                                      # without gradients nothing stands in the way
+        free = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(free):
+            y = layer_norm(x)
+        free.replay()
+        assert torch.equal(y, held[0])
+    del held
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer_norm(x), x, dy)[0], torch.autograd.grad(grouped_linear(x, w, off), (x, w), dz)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and all(torch.equal(a, b) for a, b in zip(got[1], want[1]))
+
+
+def test_streams_of_the_callers_choice():
+    """two calls at once on two streams, forward and backward on the stream that is current"""
+    from uemda_amd.norm import layer_norm
+    sets = [data(2000, 384, torch.float32, 50 + k) for k in range(2)]
+    want = []
+    for x, w, b, dy in sets:
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        y = layer_norm(*leaves)
+        want.append([y.detach()] + list(torch.autograd.grad(y, leaves, dy)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(3):
+        got = []
+        for st, (x, w, b, dy) in zip(streams, sets):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+                y = layer_norm(*leaves)
+                got.append([y.detach()] + list(torch.autograd.grad(y, leaves, dy)))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for g, v in zip(got, want) for a, c in zip(g, v))
+
+
 def test_results_repeat_and_a_captured_step_replays():
     from uemda_amd.norm import layer_norm
     x, w, b, dy = data(4097, 320, torch.bfloat16, 17)

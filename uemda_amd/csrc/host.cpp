@@ -6,6 +6,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -13,7 +14,7 @@
 #include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
-#include <limits>
+#include <optional>
 #include <sstream>
 #include <string>
 #include <utility>
@@ -72,6 +73,20 @@ void need_gpu(std::initializer_list<const Tensor*> list) {
 void no_second_derivative(const char* what) {
     // its kernels are nothing autograd can see through: under create_graph=True the result would silently count as a constant
     if (at::GradMode::is_enabled()) refuse(what, ": a gradient of the gradient is not offered (create_graph=True)");
+}
+
+// A graph of the same leaves that lives outside a capture holds the nodes that add up their gradients, on the stream they were made on; a
+// backward pass captured on another stream would join that stream to the capture, inside the engine, which ends the process.
+void no_outside_graph(const char* what, std::initializer_list<const Tensor*> list) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : list) {
+        if (!wants_grad(*t) || !t->is_leaf()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto st = node ? node->stream() : std::nullopt;
+        if (st && st->id() != c10::hip::getCurrentHIPStream(t->get_device()).id())
+            refuse(what, ": a graph of the same leaf, made outside this capture, is still alive (an output of an eager pass that somebody holds): "
+                         "release it before capturing a pass that records gradients");
+    }
 }
 
 // an argument that may be absent, as autograd takes it: absent ones have no edge in the graph
@@ -139,7 +154,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
     if (!is_real(x)) refuse("layer_norm: x must be a float32 or bfloat16 tensor, got ", x.scalar_type());
     need_gpu({&x, &w, &b});
     if (x.dim() == 0 || x.size(-1) == 0) refuse("layer_norm: x needs a last dimension of at least one channel, got shape ", x.sizes());
-    if (x.size(-1) > std::numeric_limits<int>::max()) refuse("layer_norm: more than 2^31 - 1 channels");
+    if (x.size(-1) > (1 << 30)) refuse("layer_norm: at most 2^30 channels, got ", x.size(-1));
     if (!(eps >= 0) || std::isinf(eps)) refuse("layer_norm: eps must be finite and not negative, got ", eps);
     for (const auto& [name, p] : {std::pair<const char*, const Tensor*>{"weight", &w}, {"bias", &b}})
         if (p->defined() && (p->dim() != 1 || p->size(0) != x.size(-1) || !is_real(*p) || !p->is_contiguous() || p->device() != x.device()))
@@ -147,7 +162,11 @@ Tensor layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
                    p->scalar_type(), " ", p->sizes(), " strides ", p->strides(), " on ", p->device());
     if (w.defined() && b.defined() && w.scalar_type() != b.scalar_type())
         refuse("layer_norm: weight and bias must have one type, got ", w.scalar_type(), " and ", b.scalar_type());
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) return LayerNormFn::apply(x, maybe(w), maybe(b), eps);
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(b))) {
+        const c10::DeviceGuard guard(x.device());
+        no_outside_graph("layer_norm", {&x, &w, &b});
+        return LayerNormFn::apply(x, maybe(w), maybe(b), eps);
+    }
     return norm_forward(x, w, b, eps, false).first;
 }
 
@@ -246,7 +265,11 @@ Tensor grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& offse
     if (T >= (1 << 30) || G >= (1 << 16) || std::max(K, N) > (1 << 20))
         refuse("grouped_linear: fewer than 2^30 rows and 2^16 groups and at most 2^20 channels, got ", T, ", ", G, ", ", std::max(K, N));
     const Tensor off = offsets.contiguous(), b = bias.defined() ? bias.contiguous() : bias;
-    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(b))) return GroupedLinearFn::apply(x, weight, off, maybe(b));
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(weight) || wants_grad(b))) {
+        const c10::DeviceGuard guard(x.device());
+        no_outside_graph("grouped_linear", {&x, &weight, &bias});
+        return GroupedLinearFn::apply(x, weight, off, maybe(b));
+    }
     return grouped_forward(x, weight, off, b).y;
 }
 

@@ -481,12 +481,12 @@ int run(LnP p, bool bwd, hipStream_t st) {
 }  // namespace
 
 extern "C" int64_t uem_layernorm_workspace_floats(int64_t rows, int C) {
-    int64_t nb = rows < LN_BWD_BLOCKS ? uem_cdiv(rows, 8) * 8 : LN_BWD_BLOCKS;
-    return nb * 2 * (int64_t)C;
+    const int64_t most = C > 8192 ? 64 : LN_BWD_BLOCKS;                        // longer rows: the pass over columns
+    return (rows < most ? uem_cdiv(rows, 8) * 8 : most) * 2 * (int64_t)C;
 }
 extern "C" int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
                                  int64_t rows, int C, float eps, int flags, void* stream) {
-    UEM_REQUIRE(x && y && rows > 0 && C > 0 && x_ld >= C, "layernorm_fwd: bad arguments (rows, C > 0, x_ld >= C)");
+    UEM_REQUIRE(x && y && rows > 0 && C > 0 && C <= (1 << 30) && x_ld >= C, "layernorm_fwd: bad arguments (rows > 0, 0 < C <= 2^30, x_ld >= C)");
     UEM_REQUIRE((mean == nullptr) == (rstd == nullptr), "layernorm_fwd: mean and rstd go together");
     UEM_REQUIRE((flags & ~(UEM_LN_BF16 | UEM_LN_PARAM_BF16)) == 0, "layernorm_fwd: unknown flags %d", flags);
     LnP p{};
@@ -499,8 +499,8 @@ extern "C" int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma,
 extern "C" int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld, const void* gamma, const float* mean,
                                  const float* rstd, void* dx, void* dgamma, void* dbeta, float* workspace, int64_t rows, int C, int flags,
                                  void* stream) {
-    UEM_REQUIRE(x && dy && mean && rstd && dx && rows > 0 && C > 0 && x_ld >= C && dy_ld >= C,
-                "layernorm_bwd: bad arguments (rows, C > 0, strides >= C)");
+    UEM_REQUIRE(x && dy && mean && rstd && dx && rows > 0 && C > 0 && C <= (1 << 30) && x_ld >= C && dy_ld >= C,
+                "layernorm_bwd: bad arguments (rows > 0, 0 < C <= 2^30, strides >= C)");
     UEM_REQUIRE((dgamma == nullptr && dbeta == nullptr) || workspace, "layernorm_bwd: parameter gradients need the workspace");
     UEM_REQUIRE((flags & ~(UEM_LN_BF16 | UEM_LN_PARAM_BF16)) == 0, "layernorm_bwd: unknown flags %d", flags);
     LnP p{};
