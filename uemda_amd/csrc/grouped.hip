@@ -187,6 +187,10 @@ struct Loader {
             }
         }
     }
+    // piece j of stage `q`, all of whose reduction indices exist (a KC row past the operand's end lies past the descriptor's)
+    __device__ __forceinline__ void issue_whole(int j, const i32x4 rs, char* img, int wave, int q) const {
+        uem_raw_buffer_load_lds(rs, (lds_u32p)(img + (j * NW + wave) * 1024), 16, (int)off[j], KS ? 0 : q * 64, 0, 0);
+    }
     // piece j of stage `q` of a reduction of `red`
     __device__ __forceinline__ void issue(int j, const i32x4 rs, char* img, int wave, int q, int red) const {
         const unsigned o = KS ? off[j] : (q * (64 / ES) + kc[j] < red ? off[j] + (unsigned)q * 64u : GG_OOB);
@@ -326,7 +330,9 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
         if (lane < NT * 32 && c < p.N) bias = p.bias16 ? __uint_as_float((uint32_t)((const bf16_t*)p.bias)[i] << 16) : ((const float*)p.bias)[i];
     }
 
-    // One operand's stage `q`, or stages `q` and `q` + 1; those past the end fetch zeros, so that the waits' counts hold
+    // One operand's stage `q`, or stages `q` and `q` + 1; those past the end fetch zeros, so that the waits' counts hold.
+    // Stages that lie wholly inside the reduction are sent without a check a lane, by the eight waves alone: 65536 x 2048 x 2048
+    // in 32 groups gains 1 to 2 %, and the four waves' schedule, which has no phase of its own for it, loses 5 to 8 %.
     auto desc = [](const char* b, int rem, int64_t ld, unsigned bytes, bool ks) {
         const int n = ks && rem > BK ? BK : rem;
         return rsrc(b, n > 0 ? (unsigned)((n - 1) * ld) + bytes : 0u);
@@ -334,20 +340,36 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     int qa = 0, qb = 0;                                                        // next stages to send off
     auto issue_a = [&](char* __restrict__ fill0, char* __restrict__ fill1, const bool two) {
         const i32x4 r0_ = desc(pa, arem, p.lda, acols, AKS);
+        if (AKS || (PP && (qa + (two ? 2 : 1)) * BK <= red)) {
 #pragma unroll
-        for (int j = 0; j < LA::IPW; ++j) {
-            la.issue(j, r0_, fill0, wave, qa, red);
-            if (two) la.issue(j, r0_, fill1, wave, qa + 1, red);
+            for (int j = 0; j < LA::IPW; ++j) {
+                la.issue_whole(j, r0_, fill0, wave, qa);
+                if (two) la.issue_whole(j, r0_, fill1, wave, qa + 1);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < LA::IPW; ++j) {
+                la.issue(j, r0_, fill0, wave, qa, red);
+                if (two) la.issue(j, r0_, fill1, wave, qa + 1, red);
+            }
         }
         if (AKS) { pa += BK * p.lda; arem -= BK; }
         qa += two ? 2 : 1;
     };
     auto issue_b = [&](char* __restrict__ fill0, char* __restrict__ fill1, const bool two) {
         const i32x4 r0_ = desc(pb, brem, p.ldb, bcols, BKS);
+        if (BKS || (PP && (qb + (two ? 2 : 1)) * BK <= red)) {
 #pragma unroll
-        for (int j = 0; j < LB::IPW; ++j) {
-            lb.issue(j, r0_, fill0 + BM * 64, wave, qb, red);
-            if (two) lb.issue(j, r0_, fill1 + BM * 64, wave, qb + 1, red);
+            for (int j = 0; j < LB::IPW; ++j) {
+                lb.issue_whole(j, r0_, fill0 + BM * 64, wave, qb);
+                if (two) lb.issue_whole(j, r0_, fill1 + BM * 64, wave, qb + 1);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < LB::IPW; ++j) {
+                lb.issue(j, r0_, fill0 + BM * 64, wave, qb, red);
+                if (two) lb.issue(j, r0_, fill1 + BM * 64, wave, qb + 1, red);
+            }
         }
         if (BKS) { pb += BK * p.ldb; brem -= BK; }
         qb += two ? 2 : 1;
@@ -398,6 +420,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
         if (PP) {
             fetch(0);
             fetch(1);
+            __builtin_amdgcn_sched_barrier(0);                                 // the reads first: the sends' addresses are made in their shadow
             issue(fill3, fill4, odd);
             gg_wait<FLIGHT>();
             if (FORM == WGRAD) add_up();
