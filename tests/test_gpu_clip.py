@@ -100,6 +100,9 @@ def test_layouts():
         clip_grad_norm_(params_of([a, a]), 1.0)
     with pytest.raises(UemError, match="share memory"):
         clip_grad_norm_(params_of([a[:60], a[59:]]), 1.0)
+    for pair in ([wide[:, :37], wide[:, :37]], [wide[:, :37], wide[:, 36:]], [wide[:, :37], wide[0, 30:40]]):      # with gaps: scaled in copies
+        with pytest.raises(UemError, match="overlaps"):
+            clip_grad_norm_(params_of(pair), 1.0)
     keep = a.clone()
     check([a[:60], a[60:]], 1.0)
     assert not torch.equal(a, keep)

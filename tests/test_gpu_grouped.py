@@ -122,6 +122,29 @@ def test_master_weights_int64_offsets_and_no_bias():
     check(x, w, b, dy, o, torch.int64)
 
 
+def test_master_weights_with_gaps():
+    """fp32 weights that are a slice of a wider buffer, under bf16 rows: rounded row by row, what lies between is not read"""
+    o = edges(200, [60, 0, 100], 7)
+    x, w, b, dy = data(200, 3, 48, 56, torch.bfloat16, 1, wdtype=torch.float32)
+    wide = torch.full((3, 56, 53), float("nan"), device="cuda")
+    wide[:, :, 2:50] = w
+    tall = torch.full((3, 60, 48), float("nan"), device="cuda")
+    tall[:, 3:59] = w
+    y0, g0 = check(x, w, b, dy, o)
+    for v in (wide[:, :, 2:50], tall[:, 3:59], w.transpose(1, 2).contiguous().transpose(1, 2)):
+        y, g = check(x, v, b, dy, o)
+        assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(g, g0))
+
+
+@pytest.mark.parametrize("T,G", [(5, 300), (1, 64), (70, 2000)])
+def test_fewer_rows_than_groups(T, G):
+    lens = [0] * G
+    for r in range(T):
+        lens[(r * 37 + 11) % G] += 1
+    x, w, b, dy = data(T, G, 64, 40, torch.bfloat16, G)
+    check(x, w, b, dy, edges(T, lens))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides_and_starts(dtype):
     """rows and gradients that are slices of wider buffers, transposed, or start off the 16-byte grid; nothing outside them is read in"""

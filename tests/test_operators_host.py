@@ -63,6 +63,11 @@ def test_gradient_norm_refusals():
         clip_grad_norm_([p], float("nan"))
     with pytest.raises(UemError, match="expected tensors"):
         get_total_norm([1.0])
+    with torch.inference_mode():
+        frozen = torch.ones(3)
+    p.grad = frozen
+    with pytest.raises(UemError, match="inference"):
+        clip_grad_norm_([p], 1.0)
     p.grad = torch.ones(3).to_sparse()
     with pytest.raises(UemError, match="dense"):
         clip_grad_norm_([p], 1.0)
@@ -106,3 +111,10 @@ def test_grouped_linear_refusals():
     assert lib.uem_grouped_pad(16, 4, 16, 8, 6, 4, 0, None) == -1
     for T, G, K, N in ((1, 1, 1, 1), (100, 3, 5, 7), (1 << 20, 64, 2048, 2048), (1 << 20, 2, 8, 8)):
         assert lib.uem_grouped_wgrad_workspace_floats(T, G, K, N) >= (0 if T < 1000 else N * (K + 1))
+
+
+def test_the_host_extension_needs_its_binding():
+    import subprocess
+    import sys
+    code = "import torch\nfrom uemda_amd import _host\ntry:\n    _host.layer_norm(torch.zeros(2, 8), None, None, 1e-5)\nexcept RuntimeError as e:\n    assert 'bound' in str(e)\nelse:\n    raise SystemExit(1)"
+    assert subprocess.run([sys.executable, "-c", code]).returncode == 0

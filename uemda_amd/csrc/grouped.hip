@@ -698,13 +698,13 @@ bool few_rows(const GgP& p, int es) { return likely_tiles(p.T, p.G, 32) * uem_cd
 template <typename T, int FORM>
 int launch_rows(const GgP& p, const char* what, hipStream_t st) {
     if (FORM == FWD && few_rows(p, sizeof(T))) {
-        const int64_t items = (p.T / 32 + (int64_t)p.G) * uem_cdiv(p.N, 32);
+        const int64_t items = (p.T / 32 + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(p.N, 32);
         constexpr int LDS = 16 * 32 * 36 * 4;
         if (uem_allow_lds((const void*)grouped_few_kernel<T>, LDS)) grouped_few_kernel<T><<<(unsigned)(uem_cdiv(items, 8) * 8), 1024, LDS, st>>>(p);
         return uem_check_launch(what);
     }
     const int width = FORM == FWD ? p.N : p.K, t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
-    const int64_t items = (p.T / TILES[t].bm + (int64_t)p.G + 1) * uem_cdiv(width, TILES[t].bn);     // at most so many tiles
+    const int64_t items = (p.T / TILES[t].bm + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(width, TILES[t].bn);   // at most so many tiles: one of each group with rows is not full
     UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than the kernels count", what, (long long)items);
     if (t == 0) go<T, FORM, 256, 256, 2, 4>(p, items, st);
     else if (t == 1) go<T, FORM, 128, 128, 2, 2>(p, items, st);

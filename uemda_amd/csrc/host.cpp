@@ -6,6 +6,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/InferenceMode.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -13,6 +14,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <sstream>
@@ -195,6 +197,7 @@ Grouped grouped_forward(const Tensor& x, const Tensor& weight, const Tensor& off
     if (T == 0) return r;
     Tensor w = weight.reshape({G * N, K});
     if (w.scalar_type() != x.scalar_type()) {                                  // fp32 master weights under bf16 rows
+        w = w.contiguous();
         const Tensor w16 = at::empty({G * N, K}, x.options());
         CALL(uem_cast_f32_bf16, w.const_data_ptr<float>(), (uint16_t*)mptr(w16), w.numel(), stream_of(x));
         w = w16;
@@ -283,17 +286,25 @@ Tensor multi_norm(std::vector<Tensor> list, const std::string& what, int kind, b
     std::vector<int64_t> numels(n);
     std::vector<uint8_t> kinds(n);
     std::vector<std::pair<Tensor, Tensor>> copies;
+    std::vector<std::pair<uint64_t, uint64_t>> spans;                         // of the gradients themselves
     for (int i = 0; i < n; ++i) {
         Tensor& t = list[i];
         if (t.layout() != at::kStrided) refuse(what, ": gradients must be dense tensors, got ", t.layout());
+        if (clip && t.is_inference() && !c10::InferenceMode::is_enabled()) refuse(what, ": a gradient is an inference tensor: it cannot be scaled in place");
         if (!is_real(t)) refuse(what, ": gradients must be float32 or bfloat16 tensors, got ", t.scalar_type());
         if (t.device() != dev || !t.is_cuda())
             refuse(what, ": all gradients must be on one MI355X device, got ", dev, " and ", t.device(), " (there is no CPU / PyTorch fallback)");
+        if (clip && t.numel() > 0) {
+            uint64_t last = 0;                                                 // from its first element
+            for (int64_t d = 0; d < t.dim(); ++d) {
+                if (t.stride(d) == 0 && t.size(d) > 1)
+                    refuse(what, ": a gradient of shape ", t.sizes(), ", strides ", t.strides(), " repeats its elements: it cannot be scaled in place");
+                last += (uint64_t)(t.size(d) - 1) * t.stride(d);
+            }
+            const uint64_t first = (uint64_t)t.const_data_ptr();
+            spans.emplace_back(first, first + (last + 1) * t.element_size());
+        }
         if (!t.is_non_overlapping_and_dense()) {                               // gaps between its elements: summed, and scaled, in a dense copy
-            if (clip)
-                for (int64_t d = 0; d < t.dim(); ++d)
-                    if (t.stride(d) == 0 && t.size(d) > 1)
-                        refuse(what, ": a gradient of shape ", t.sizes(), ", strides ", t.strides(), " repeats its elements: it cannot be scaled in place");
             Tensor c = t.contiguous();
             if (clip) copies.emplace_back(t, c);
             t = c;
@@ -301,6 +312,11 @@ Tensor multi_norm(std::vector<Tensor> list, const std::string& what, int kind, b
         ptrs[i] = (uint64_t)t.const_data_ptr();
         numels[i] = t.numel();
         kinds[i] = is16(t) ? 1 : 0;
+    }
+    if (!copies.empty()) {                                                     // (the library sees the copies only)
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            if (spans[i].first < spans[i - 1].second) refuse(what, ": the memory of two gradients overlaps or interleaves: they cannot be scaled in place");
     }
     const c10::DeviceGuard guard(dev);
     const auto opt = list[0].options();
@@ -327,6 +343,10 @@ double double_arg(PyObject* o) {
     return v;
 }
 void count_args(const char* what, Py_ssize_t got, Py_ssize_t want) {
+    if (uem_grouped_wgrad_ == nullptr) {
+        PyErr_SetString(PyExc_RuntimeError, "uemda_amd._host is not bound to the library: uemda_amd._lib.host() does that");
+        throw python_error();
+    }
     if (got != want) refuse(what, ": ", want, " arguments expected, got ", got);
 }
 PyObject* py_layer_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
