@@ -141,20 +141,35 @@ struct Groups {
         t.tile = target - t.before;
         return t;
     }
-    // the tiles of group `g`
-    __device__ __forceinline__ Tile of(const GgP& p, int bm, int lane, int g, int& n) {
-        Tile t{};
+    // the k-th of the groups of several tiles; false if there are not so many.  n: its tiles
+    __device__ __forceinline__ bool several(const GgP& p, int bm, int lane, int k, Tile& t, int& n) {
         int edge = __builtin_amdgcn_readfirstlane(gg_offset(p, 0)), ntiles = 0, nslot = 0;
-        for (int c = 0; c * 64 <= g; ++c) load(p, bm, c, lane, edge, ntiles, nslot);
-        pick(g & 63, t);
-        n = lane_value(nt, g & 63);
-        return t;
+        for (int c = 0; c * 64 < p.G; ++c) {
+            load(p, bm, c, lane, edge, ntiles, nslot);
+            unsigned long long m = __ballot(nt > 1);
+            const int here = __popcll(m);
+            if (k >= here) { k -= here; continue; }
+            for (; k > 0; --k) m &= m - 1;
+            const int l = __builtin_ctzll(m);
+            pick(l, t);
+            n = lane_value(nt, l);
+            return true;
+        }
+        return false;
     }
 };
 // Blocks go to the eight XCDs in turn: each XCD gets one contiguous run of the n items, neighbours share operand tiles in its L2.
 __device__ __forceinline__ int xcd_item(int n) {
     const int x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rem = n & 7;
     return i < per + (x < rem ? 1 : 0) ? x * per + (x < rem ? x : rem) + i : -1;
+}
+
+// Weight gradient: tile p of a group's rt x ct goes to XCD p & 7 (where rt * ct is a multiple of eight)
+__device__ __forceinline__ int spread_tiles(int p, int rt, int ct) {
+    const int x = p & 7, l = p >> 3;
+    if ((rt & 3) == 0 && (ct & 1) == 0) return ((x >> 1) * (rt >> 2) + l / (ct >> 1)) * ct + (x & 1) * (ct >> 1) + l % (ct >> 1);
+    if ((rt & 1) == 0 && (ct & 3) == 0) return ((x >> 2) * (rt >> 1) + l / (ct >> 2)) * ct + (x & 3) * (ct >> 2) + l % (ct >> 2);
+    return p;
 }
 
 // ---- operand images -------------------------------------------------------------------------------------------------------------------
@@ -236,16 +251,15 @@ template <int R> struct Frag<float, true, R> {
 template <typename FA, typename FB> __device__ __forceinline__ void mma(const FA& a, const FB& b, f32x16& c, bf16_t) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0);
 }
-// sum of a lane's elements of a fragment (on the vector units, which the matrix cores leave idle)
-template <typename FA> __device__ __forceinline__ float sum_of(const FA& a, bf16_t) {
-    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    const u32x4 u = __builtin_bit_cast(u32x4, a.v);
-    float s[4];
+// a lane's elements of a fragment added to s, on the vector units (bf16 two at a time, as products with ones)
+template <typename FA> __device__ __forceinline__ float add_of(const FA& a, float s, bf16_t) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = __uint_as_float(u[i] << 16) + __uint_as_float(u[i] & 0xffff0000u);
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a.v[2 * i], a.v[2 * i + 1]}, ones, s, false);
+    return s;
 }
-template <typename FA> __device__ __forceinline__ float sum_of(const FA& a, float) { return (a.v[0] + a.v[1]) + (a.v[2] + a.v[3]); }
+template <typename FA> __device__ __forceinline__ float add_of(const FA& a, float s, float) { return s + ((a.v[0] + a.v[1]) + (a.v[2] + a.v[3])); }
 template <typename FA, typename FB> __device__ __forceinline__ void mma(const FA& a, const FB& b, f32x16& c, float) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[e], b.v[e], c, 0, 0, 0);
@@ -302,12 +316,14 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     groups.init(p, bm, lane);
 
     if (FORM != WGRAD) zero_rows<64 * NW>(p, groups, width);
-    const int item = xcd_item(groups.total * ct * rt);
+    const int item = FORM == WGRAD ? ((int)blockIdx.x < groups.total * ct * rt ? (int)blockIdx.x : -1) : xcd_item(groups.total * ct * rt);
     if (item < 0) return;
 
     // ---- the tile
     const Tile tl = groups.find(p, bm, lane, item / (ct * rt));
-    const int within = item % (ct * rt), c0 = (within % ct) * BN, n0 = (within / ct) * BM;      // n0: first row of W (WGRAD)
+    int within = item % (ct * rt);
+    if (FORM == WGRAD) within = spread_tiles(within, rt, ct);
+    const int c0 = (within % ct) * BN, n0 = (within / ct) * BM;                // n0: first row of W (WGRAD)
     const int r0 = tl.row0 + tl.tile * bm;
     int rows = tl.rows - tl.tile * bm;                                         // feature rows of the tile
     rows = rows < 0 ? 0 : rows < bm ? rows : bm;
@@ -413,7 +429,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
             if (!sums) return;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                if (i == wave % WGN) colsum += sum_of(fa[0][i], T{}) + sum_of(fa[1][i], T{});
+                if (i == wave % WGN) colsum = add_of(fa[1][i], add_of(fa[0][i], colsum, T{}), T{});
         };
         // In front of stage t (PP: in stage t - 1, behind its sends) the pieces of stage t have to have landed.  Newer than the last of them
         // are, of a KS operand, three stages' pieces and, of a KC operand, those of the pair behind its own (and, t even, its partner's last).
@@ -608,34 +624,45 @@ __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
     else reinterpret_cast<float*>(p.out)[at] = v;
 }
 
-// dW and db of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: group
+// the sum of n values `step` apart, in their order, four of them on the way at a time
+template <typename V> __device__ __forceinline__ V sum_in_order(const V* p, int64_t step, int n) {
+    V v = *p;
+    int c = 1;
+    for (; c + 3 < n; c += 4) {
+        V u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = p[(c + k) * step];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v += u[k];
+    }
+    for (; c < n; ++c) v += p[c * step];
+    return v;
+}
+// dW and db of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: which of those groups
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
-    const int g = blockIdx.y;
     int n;
+    Tile t{};
     Groups<true> groups;
-    const Tile t = groups.of(p, p.chunk, threadIdx.x & 63, g, n);
-    if (n <= 1) return;
+    if (!groups.several(p, p.chunk, threadIdx.x & 63, blockIdx.y, t, n)) return;
+    const int g = t.group;
     const int64_t size = (int64_t)p.N * p.K;
     const float* const part = p.part + t.slot * size;
     if (p.vec && (size & 3) == 0) {                                            // rows of whole 16-byte stores: so is the whole of dW_g
         for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
-            f32x4 v = *reinterpret_cast<const f32x4*>(part + i);
-            for (int c = 1; c < n; ++c) v += *reinterpret_cast<const f32x4*>(part + c * size + i);
+            const f32x4 v = sum_in_order(reinterpret_cast<const f32x4*>(part + i), size / 4, n);
             if (p.out16) *reinterpret_cast<uint2*>(p.out + (g * size + i) * 2) = make_uint2(bf_bits(v[0]) | (bf_bits(v[1]) << 16), bf_bits(v[2]) | (bf_bits(v[3]) << 16));
             else *reinterpret_cast<f32x4*>(p.out + (g * size + i) * 4) = v;
         }
     } else {
         for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-            float v = part[i];
-            for (int c = 1; c < n; ++c) v += part[c * size + i];
+            const float v = sum_in_order(part + i, size, n);
             if (p.out16) reinterpret_cast<bf16_t*>(p.out)[g * size + i] = (bf16_t)bf_bits(v);
             else reinterpret_cast<float*>(p.out)[g * size + i] = v;
         }
     }
     if (p.db != nullptr)
         for (int c = blockIdx.x * 256 + threadIdx.x; c < p.N; c += gridDim.x * 256) {
-            float v = 0.f;
-            for (int k = 0; k < n; ++k) v += p.part_db[(int64_t)(t.slot + k) * p.N + c];
+            const float v = sum_in_order(p.part_db + (int64_t)t.slot * p.N + c, p.N, n);
             if (p.bias16) ((bf16_t*)p.db)[(int64_t)g * p.N + c] = (bf16_t)bf_bits(v);
             else ((float*)p.db)[(int64_t)g * p.N + c] = v;
         }
@@ -794,7 +821,8 @@ extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x
     else go<float, WGRAD, 128, 128, 2, 2>(p, items, st);
     if (slots > 0) {
         const int64_t nb = uem_cdiv((int64_t)N * K, 1024);
-        grouped_join_kernel<<<dim3((unsigned)(nb < 512 ? nb : 512), (unsigned)G), 256, 0, st>>>(p);
+        const int64_t most = slots / 2 < G ? slots / 2 : G;                    // groups of several chunks
+        grouped_join_kernel<<<dim3((unsigned)(nb < 512 ? nb : 512), (unsigned)most), 256, 0, st>>>(p);
     }
     return uem_check_launch("grouped_wgrad");
 }

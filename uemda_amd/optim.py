@@ -32,6 +32,7 @@ def get_total_norm(tensors, norm_type=2.0):
     """The norm over all elements of all `tensors` (a tensor or an iterable; fp32 and bf16 may be mixed), as a 0-dim fp32 device tensor:
     torch.nn.utils.get_total_norm for norm_type 2 or inf.  Squares are summed in 64 bits, in a fixed order; no value is read on the host."""
     what = "get_total_norm"
+    ops.grad_join()                # gradients of arena parameters among them may still be on the side / second stream
     norm = _lib.host().multi_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), what, _norm_kind(norm_type, what), False, None)
     return torch.tensor(0.0) if norm is None else norm
 
