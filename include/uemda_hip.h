@@ -512,7 +512,7 @@ int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld
  * fp32 master weight); bias / db are fp32, or bf16 with UEM_GROUPED_BIAS_BF16.  *_ld: row strides in ELEMENTS; rows of the operands must
  * begin on 16-byte boundaries and be followed by zeros up to the next one (whatever their stride holds beyond it) -- uem_grouped_pad copies
  * rows of any length to such a stride.  No group is read beyond its
- * rows, sums run in a fixed order.                                                                                                */
+ * rows, sums run in a fixed order.  A size of the workspace goes with the flags of the call.                                      */
 #define UEM_GROUPED_BF16 1
 #define UEM_GROUPED_OUT_F32 2
 #define UEM_GROUPED_BIAS_BF16 4
@@ -522,7 +522,7 @@ int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void
                     int flags, void* stream);
 int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w_ld, void* dx, const void* offsets, int T, int G, int K, int N, int flags,
                       void* stream);
-int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N);
+int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N, int flags);
 int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x_ld, void* dw, void* db, float* workspace, const void* offsets, int T, int G,
                       int K, int N, int flags, void* stream);
 

@@ -110,7 +110,7 @@ def test_grouped_linear_refusals():
     assert lib.uem_grouped_wgrad(16, 8, 16, 8, 16, 16, None, 16, 1 << 20, 2, 8, 8, 0, None) == -1 and b"workspace" in lib.uem_last_error()
     assert lib.uem_grouped_pad(16, 4, 16, 8, 6, 4, 0, None) == -1
     for T, G, K, N in ((1, 1, 1, 1), (100, 3, 5, 7), (1 << 20, 64, 2048, 2048), (1 << 20, 2, 8, 8)):
-        assert lib.uem_grouped_wgrad_workspace_floats(T, G, K, N) >= (0 if T < 1000 else N * (K + 1))
+        assert lib.uem_grouped_wgrad_workspace_floats(T, G, K, N, 0) >= (0 if T < 1000 else N * (K + 1))
 
 
 def test_the_host_extension_needs_its_binding():

@@ -153,7 +153,7 @@ SIGNATURES = {
     "uem_grouped_pad": [P, L, P, I, I, L, I, P],
     "uem_grouped_fwd": [P, I, P, I, P, P, P, I, I, I, I, I, P],
     "uem_grouped_dgrad": [P, I, P, I, P, P, I, I, I, I, I, P],
-    "uem_grouped_wgrad_workspace_floats": [I, I, I, I],
+    "uem_grouped_wgrad_workspace_floats": [I, I, I, I, I],
     "uem_grouped_wgrad": [P, I, P, I, P, P, P, P, I, I, I, I, I, P],
     "uem_comm_unique_id": [P],
     "uem_comm_init": [POINTER(c_void_p), P, I, I],

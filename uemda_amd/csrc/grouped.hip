@@ -89,70 +89,91 @@ __device__ __forceinline__ int scan_max(int v) {   // v >= 0
 }
 __device__ __forceinline__ int lane_value(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
-// The groups cut into tiles of `bm` rows, 64 groups at a time, one a lane.  ONE: an empty group still has a tile (which writes its zeros).
-// `slot`: groups of several tiles take that many slots for partial sums, the others none.
-struct Tile { int group, row0, rows, tile, before, slot; };       // rows: of the whole group; before: tiles of the groups in front of it
-template <bool ONE>
+// The groups cut into tiles of `bm` rows, 64 groups at a time, one a lane, numbered in row order.
+// LPT (the weight gradient's chunks): an empty group has a tile too (which writes its zeros), and the tiles are numbered whole ones first,
+// then the groups' rests, the longest first: what comes last on the chip is short, however the rows fall to the groups.
+struct Tile { int group, row0, rows, tile, tiles, slot; };        // rows, tiles: of the whole group
+template <bool LPT>
 struct Groups {
-    int begin, len, nt, tiles, slots;             // of the lane's group; tiles, slots: up to and with it
+    int begin, len, nt, count, slots;             // of the lane's group; count, slots: tiles (LPT: whole ones) and slots up to and with it.
+    bool rest;                                    // LPT: it has a tile that is not whole.  Groups of several tiles take as many slots
     int loaded;                                   // which 64 groups the lanes hold
-    int first, last, total, nslots;               // rows of all groups: [first, last); tiles and slots in all
-    __device__ __forceinline__ void load(const GgP& p, int bm, int chunk, int lane, int& edge, int& ntiles, int& nslot) {
+    int first, last, total, rests;                // rows of all groups: [first, last); tiles (whole ones, rests) in all
+    __device__ __forceinline__ void load(const GgP& p, int bm, int chunk, int lane, int& edge, int& before, int& nslot) {
         const int v = chunk * 64 + lane;
         int end = v < p.G ? gg_offset(p, v + 1) : 0;
         end = scan_max(end > edge ? end : edge);
         const int up = __shfl_up(end, 1, 64);
         begin = lane == 0 ? edge : up;
         len = end - begin;
-        nt = v < p.G ? (len + bm - 1) / bm : 0;
-        if (ONE && v < p.G && nt == 0) nt = 1;
-        tiles = scan_add(nt) + ntiles;
-        slots = ONE ? scan_add(nt > 1 ? nt : 0) + nslot : 0;
+        const int whole = v < p.G ? len / bm : 0;
+        rest = v < p.G && (len > whole * bm || (LPT && len == 0));
+        nt = whole + (rest ? 1 : 0);
+        count = scan_add(LPT ? whole : nt) + before;
+        slots = LPT ? scan_add(nt > 1 ? nt : 0) + nslot : 0;
         loaded = chunk;
         edge = lane_value(end, 63);
-        ntiles = lane_value(tiles, 63);
-        nslot = ONE ? lane_value(slots, 63) : 0;
+        before = lane_value(count, 63);
+        nslot = LPT ? lane_value(slots, 63) : 0;
     }
     __device__ __forceinline__ void init(const GgP& p, int bm, int lane) {
         first = __builtin_amdgcn_readfirstlane(gg_offset(p, 0));
         last = first;
-        total = nslots = 0;
-        for (int c = 0; c * 64 < p.G; ++c) load(p, bm, c, lane, last, total, nslots);
+        total = rests = 0;
+        int nslot = 0;
+        for (int c = 0; c * 64 < p.G; ++c) {
+            load(p, bm, c, lane, last, total, nslot);
+            if (LPT) rests += __popcll(__ballot(rest));
+        }
     }
-    __device__ __forceinline__ bool pick(int l, Tile& t) const {
+    __device__ __forceinline__ Tile pick(int l) const {
+        Tile t;
         t.group = loaded * 64 + l;
-        t.before = lane_value(tiles, l) - lane_value(nt, l);
         t.row0 = lane_value(begin, l);
         t.rows = lane_value(len, l);
-        t.slot = ONE ? lane_value(slots, l) - (lane_value(nt, l) > 1 ? lane_value(nt, l) : 0) : 0;
-        return true;
-    }
-    // tile number `target` < total
-    __device__ __forceinline__ Tile find(const GgP& p, int bm, int lane, int target) {
-        Tile t{};
-        if (p.G > 64) {                                                        // walk the groups 64 at a time again
-            int edge = first, ntiles = 0, nslot = 0;
-            for (int c = 0; c * 64 < p.G; ++c) {
-                load(p, bm, c, lane, edge, ntiles, nslot);
-                if (ntiles > target) break;
-            }
-        }
-        pick(__builtin_ctzll(__ballot(tiles > target)), t);
-        t.tile = target - t.before;
+        t.tiles = lane_value(nt, l);
+        t.slot = LPT ? lane_value(slots, l) - (t.tiles > 1 ? t.tiles : 0) : 0;
+        t.tile = 0;
         return t;
     }
-    // the k-th of the groups of several tiles; false if there are not so many.  n: its tiles
-    __device__ __forceinline__ bool several(const GgP& p, int bm, int lane, int k, Tile& t, int& n) {
-        int edge = __builtin_amdgcn_readfirstlane(gg_offset(p, 0)), ntiles = 0, nslot = 0;
+    // tile number `target` < total + rests
+    __device__ __forceinline__ Tile find(const GgP& p, int bm, int lane, int target) {
+        const bool is_rest = LPT && target >= total;
+        if (is_rest) target -= total;
+        if (p.G > 64) {                                                        // walk the groups 64 at a time again
+            int edge = first, before = 0, nslot = 0;
+            for (int c = 0; c * 64 < p.G; ++c) {
+                load(p, bm, c, lane, edge, before, nslot);
+                if (!is_rest && before > target) break;
+                const int here = is_rest ? __popcll(__ballot(rest)) : 0;
+                if (is_rest && here > target) break;
+                target -= here;
+            }
+        }
+        if (is_rest) {                                                         // the rest with `target` longer ones among the lanes'
+            const int left = len - (nt - 1) * bm, key = rest ? (left < (1 << 25) ? left : (1 << 25) - 1) * 64 + 63 - lane : -1;
+            const int n = p.G - loaded * 64 < 64 ? p.G - loaded * 64 : 64;
+            int longer = 0;
+            for (int i = 0; i < n; ++i) longer += lane_value(key, i) > key ? 1 : 0;
+            Tile t = pick(__builtin_ctzll(__ballot(rest && longer == target)));
+            t.tile = t.tiles - 1;
+            return t;
+        }
+        const int l = __builtin_ctzll(__ballot(count > target));
+        Tile t = pick(l);
+        t.tile = target - (lane_value(count, l) - (LPT ? t.rows / bm : t.tiles));
+        return t;
+    }
+    // the k-th of the groups of several tiles; false if there are not so many
+    __device__ __forceinline__ bool several(const GgP& p, int bm, int lane, int k, Tile& t) {
+        int edge = __builtin_amdgcn_readfirstlane(gg_offset(p, 0)), before = 0, nslot = 0;
         for (int c = 0; c * 64 < p.G; ++c) {
-            load(p, bm, c, lane, edge, ntiles, nslot);
+            load(p, bm, c, lane, edge, before, nslot);
             unsigned long long m = __ballot(nt > 1);
             const int here = __popcll(m);
             if (k >= here) { k -= here; continue; }
             for (; k > 0; --k) m &= m - 1;
-            const int l = __builtin_ctzll(m);
-            pick(l, t);
-            n = lane_value(nt, l);
+            t = pick(__builtin_ctzll(m));
             return true;
         }
         return false;
@@ -316,7 +337,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     groups.init(p, bm, lane);
 
     if (FORM != WGRAD) zero_rows<64 * NW>(p, groups, width);
-    const int item = FORM == WGRAD ? ((int)blockIdx.x < groups.total * ct * rt ? (int)blockIdx.x : -1) : xcd_item(groups.total * ct * rt);
+    const int item = FORM == WGRAD ? ((int)blockIdx.x < (groups.total + groups.rests) * ct * rt ? (int)blockIdx.x : -1) : xcd_item(groups.total * ct * rt);
     if (item < 0) return;
 
     // ---- the tile
@@ -489,7 +510,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     gg_barrier();                                                              // the stages' memory takes the results
 
     // ---- results
-    const bool partial = FORM == WGRAD && tl.rows > p.chunk;                   // a chunk of a group with several: to its slot, in fp32
+    const bool partial = FORM == WGRAD && tl.tiles > 1;                   // a chunk of a group with several: to its slot, in fp32
     const int64_t ldo = FORM == WGRAD ? p.K : p.ldo;
     const int64_t first = (FORM == WGRAD ? (int64_t)(partial ? tl.slot + tl.tile : tl.group) * p.N * p.K + (int64_t)n0 * ldo : (int64_t)r0 * ldo) + wm * ldo + c0 + wn;
     const int left = (FORM == WGRAD ? p.N - n0 : rows) - wm, cols = width - c0 - wn;            // output rows and columns from the wave's first on
@@ -640,11 +661,10 @@ template <typename V> __device__ __forceinline__ V sum_in_order(const V* p, int6
 }
 // dW and db of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: which of those groups
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
-    int n;
     Tile t{};
     Groups<true> groups;
-    if (!groups.several(p, p.chunk, threadIdx.x & 63, blockIdx.y, t, n)) return;
-    const int g = t.group;
+    if (!groups.several(p, p.chunk, threadIdx.x & 63, blockIdx.y, t)) return;
+    const int g = t.group, n = t.tiles;
     const int64_t size = (int64_t)p.N * p.K;
     const float* const part = p.part + t.slot * size;
     if (p.vec && (size & 3) == 0) {                                            // rows of whole 16-byte stores: so is the whole of dW_g
@@ -709,11 +729,23 @@ int pick_tile(int T, int G, int width, bool is16) {
     return best;
 }
 int wgrad_tile(int G, int N, int K) { return uem_cdiv(N, 256) * uem_cdiv(K, 256) * G >= 96 && N > 128 && K > 128 ? 256 : 128; }
-// Rows of a weight-gradient item: about what one of the 256 blocks at work (two of them a CU with 128 x 128 tiles) has to do in all, so that a
-// group with most of the rows spreads over the chip; each slot of partial sums costs N * K * 8 bytes of traffic.  Measured, us: 26215 x (2048
-// -> 512) in 7 classes, one of them with 9679 rows, 256 x 256 tiles, 512 / 1024 / 2048 / 3648 / 8192 rows: 147 / 107 / 80 / 96 / 163.
+// Tiles of the weight gradient.  fp32: 128 x 128, two of them a CU (its products are slow enough that the larger tile's fewer operand bytes
+// gain nothing and its rounding up of N, K and the blocks' number costs up to half: 40000 x (640 -> 768) in 13 groups 682 / 340 us).
+// bf16: 256 x 256 where each of the 256 CUs has the products of 1536 rows of such a tile to do: 65536 x 2048 x 2048 in 32 groups 504 us / 618 with
+// 128 x 128, 60000 x (640 -> 768) in 5 97 / 142 (2109 rows a CU); 20000 x 1024 x 1024 in 24 76 / 60 (1250), 9000 x (2048 -> 1024) in 12 65 / 52 (1125).
+int wgrad_tile(int T, int N, int K, bool is16) { return is16 && (int64_t)T * uem_cdiv(N, 256) * uem_cdiv(K, 256) >= 1536 * 256 && N > 128 && K > 128 ? 256 : 128; }
+// Rows of a weight-gradient item: what one of the 256 blocks at work (two of them a CU with 128 x 128 tiles) has to do in all, so that a group with
+// most of the rows spreads over the chip; each slot of partial sums costs N * K * 8 bytes of traffic.  With 256 x 256 tiles a block too many is a
+// round too many: each group's rest counts as half an item, in as many rounds as leave room for the others.  32768 x (2048 -> 512) in 7 groups
+// 101 -> 91 us, 60000 x (640 -> 768) in 5 108 -> 97; with 128 x 128 tiles it loses as often as it gains.
 int wgrad_chunk(int T, int G, int N, int K, int bm) {
-    const int64_t c = uem_cdiv((int64_t)T * uem_cdiv(N, bm) * uem_cdiv(K, bm), bm == 256 ? 256 : 512);
+    const double per = (bm == 256 ? 256. : 512.) / (double)(uem_cdiv(N, bm) * uem_cdiv(K, bm));        // items of a tile in a round
+    double n = per;
+    if (bm == 256) {
+        const double rests = 0.5 * (G < T ? G : T);
+        n = ceil(rests / per + 0.5) * per - rests;
+    }
+    const int64_t c = (int64_t)ceil(T / n);
     return (int)(uem_cdiv(c < 256 ? 256 : c < T ? c : T, 64) * 64);
 }
 int64_t wgrad_slots(int T, int chunk) { return T > chunk ? 2 * (int64_t)T / chunk : 0; }      // m > 1 chunks are of more than (m - 1) * chunk rows
@@ -795,8 +827,8 @@ extern "C" int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w
     return (flags & UEM_GROUPED_BF16) ? launch_rows<bf16_t, DGRAD>(p, "grouped_dgrad", (hipStream_t)stream)
                                       : launch_rows<float, DGRAD>(p, "grouped_dgrad", (hipStream_t)stream);
 }
-extern "C" int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N) {
-    const int64_t slots = wgrad_slots(T, wgrad_chunk(T, G, N, K, wgrad_tile(G, N, K)));
+extern "C" int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N, int flags) {
+    const int64_t slots = wgrad_slots(T, wgrad_chunk(T, G, N, K, wgrad_tile(T, N, K, (flags & UEM_GROUPED_BF16) != 0)));
     return (slots * (int64_t)N * K + 3) / 4 * 4 + slots * N;
 }
 extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x_ld, void* dw, void* db, float* workspace, const void* offsets, int T,
@@ -806,7 +838,8 @@ extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x
     UEM_REQUIRE(dy_ld >= N && x_ld >= K, "grouped_wgrad: row strides shorter than the rows");
     hipStream_t st = (hipStream_t)stream;
     GgP p = params(dy, dy_ld, x, x_ld, dw, K, offsets, T, G, K, N, flags);
-    const int bm = wgrad_tile(G, N, K);
+    const bool h = (flags & UEM_GROUPED_BF16) != 0;
+    const int bm = wgrad_tile(T, N, K, h);
     p.chunk = wgrad_chunk(T, G, N, K, bm);
     const int64_t slots = wgrad_slots(T, p.chunk), items = (T / p.chunk + (int64_t)G) * uem_cdiv(N, bm) * uem_cdiv(K, bm);
     UEM_REQUIRE(slots == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "grouped_wgrad: no workspace, or not on a 16-byte boundary");
@@ -814,9 +847,7 @@ extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x
     p.db = db;
     p.part = workspace;
     p.part_db = workspace + (slots * (int64_t)N * K + 3) / 4 * 4;
-    const bool h = (flags & UEM_GROUPED_BF16) != 0;
-    if (bm == 256 && h) go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, st);
-    else if (bm == 256) go<float, WGRAD, 256, 256, 2, 4>(p, items, st);
+    if (bm == 256) go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, st);
     else if (h) go<bf16_t, WGRAD, 128, 128, 2, 2>(p, items, st);
     else go<float, WGRAD, 128, 128, 2, 2>(p, items, st);
     if (slots > 0) {

@@ -242,7 +242,7 @@ struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
             const int flags = grouped_flags(x, offsets);
             if (need_x) CALL(uem_grouped_dgrad, ptr(dy), dy_ld, ptr(w), row_stride(w), mptr(dx), ptr(offsets), T, G, K, N, flags, stream_of(x));
             if (need_w || need_b) {
-                const int64_t n = uem_grouped_wgrad_workspace_floats_(T, G, K, N);
+                const int64_t n = uem_grouped_wgrad_workspace_floats_(T, G, K, N, flags);
                 Tensor ws;
                 if (n > 0) ws = at::empty({n}, x.options().dtype(at::kFloat));
                 CALL(uem_grouped_wgrad, ptr(dy), dy_ld, ptr(x), row_stride(x), mptr(dw), mptr(db), (float*)mptr(ws), ptr(offsets), T, G, K, N,
