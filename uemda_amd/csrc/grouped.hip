@@ -714,21 +714,21 @@ void go(const GgP& p, int64_t items, hipStream_t st) {
 
 // Tile of the forward and the data gradient: the one whose slowest CU has the least to do.  The larger a tile the fewer operand bytes a
 // flop; a smaller one wastes less of a short group and spreads further.  The factors are the rates measured with every CU at work, of the
-// largest tile's: bf16 65536 x 2048 -> 2048 in 32 groups 515 / 635 / 873 us, fp32 65536 x 512 -> 512 in 8 groups 309 / 299 / 285.
+// best tile's: bf16 65536 x 2048 -> 2048 in 32 groups 500 / 597 / 845 us; fp32 65536 x 1024 -> 2048 in 32 groups 2090 / 1997 / 2104 us, and
+// at no size tried has the largest been the best in fp32 (26214 x 512 -> 512 in 7 groups 136 / 134 / 124): it is not built.
 struct TileShape { int bm, bn; double rate16, rate32; };
-constexpr TileShape TILES[3] = {{256, 256, 1.0, 1.0}, {128, 128, 0.8, 1.03}, {64, 128, 0.6, 1.08}};
+constexpr TileShape TILES[3] = {{256, 256, 1.0, 0.0}, {128, 128, 0.8, 1.0}, {64, 128, 0.6, 0.97}};
 int64_t likely_tiles(int T, int G, int bm) { return uem_cdiv(T, bm) + (G < T ? G : T) / 2; }      // half a tile of each group is empty
 int pick_tile(int T, int G, int width, bool is16) {
-    int best = 0;
+    int best = -1;
     double least = 0;
-    for (int i = 0; i < 3; ++i) {
+    for (int i = is16 ? 0 : 1; i < 3; ++i) {
         const double n = (double)uem_cdiv(likely_tiles(T, G, TILES[i].bm) * uem_cdiv(width, TILES[i].bn), 256);
         const double cost = n * TILES[i].bm * TILES[i].bn / (is16 ? TILES[i].rate16 : TILES[i].rate32);
-        if (i == 0 || cost < least) { best = i; least = cost; }
+        if (best < 0 || cost < least) { best = i; least = cost; }
     }
     return best;
 }
-int wgrad_tile(int G, int N, int K) { return uem_cdiv(N, 256) * uem_cdiv(K, 256) * G >= 96 && N > 128 && K > 128 ? 256 : 128; }
 // Tiles of the weight gradient.  fp32: 128 x 128, two of them a CU (its products are slow enough that the larger tile's fewer operand bytes
 // gain nothing and its rounding up of N, K and the blocks' number costs up to half: 40000 x (640 -> 768) in 13 groups 682 / 340 us).
 // bf16: 256 x 256 where each of the 256 CUs has the products of 1536 rows of such a tile to do: 65536 x 2048 x 2048 in 32 groups 504 us / 618 with
@@ -765,7 +765,7 @@ int launch_rows(const GgP& p, const char* what, hipStream_t st) {
     const int width = FORM == FWD ? p.N : p.K, t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
     const int64_t items = (p.T / TILES[t].bm + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(width, TILES[t].bn);   // at most so many tiles: one of each group with rows is not full
     UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than the kernels count", what, (long long)items);
-    if (t == 0) go<T, FORM, 256, 256, 2, 4>(p, items, st);
+    if (sizeof(T) == 2 && t == 0) go<bf16_t, FORM, 256, 256, 2, 4>(p, items, st);
     else if (t == 1) go<T, FORM, 128, 128, 2, 2>(p, items, st);
     else go<T, FORM, 64, 128, 1, 4>(p, items, st);
     return uem_check_launch(what);
