@@ -81,6 +81,23 @@ def test_mixed_types_at_any_element_of_one_allocation(seed):
         assert (flat[~owned.cuda()] == guard).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_tensor_of_more_than_2_to_the_31_elements(dtype):
+    from uemda_amd.optim import clip_grad_norm_
+    n = 2 ** 31 + 12345
+    t = torch.zeros(n + 1, dtype=dtype, device="cuda")[1:]                     # off the 16-byte grid
+    spots = [0, 1, 2 ** 30, 2 ** 31 - 1, 2 ** 31, n - 9, n - 1]
+    for i, s in enumerate(spots):
+        t[s] = 2.0 ** i
+    want = math.sqrt(sum(4.0 ** i for i in range(len(spots))))
+    got = clip_grad_norm_(params_of([t]), 1.0)
+    assert abs(float(got) - want) <= 2.0 ** -23 * want
+    for i, s in enumerate(spots):                                              # 5 half steps of fp32, one of the type's
+        ref = 2.0 ** i / (want + 1e-6)
+        assert abs(float(t[s]) - ref) <= ref * (5 * 2.0 ** -24 + (2.0 ** -8 if dtype == torch.bfloat16 else 0))
+    assert int(torch.count_nonzero(t)) == len(spots)
+
+
 def test_layouts():
     from uemda_amd import UemError
     from uemda_amd.optim import clip_grad_norm_, get_total_norm

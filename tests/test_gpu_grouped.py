@@ -114,6 +114,34 @@ def test_sizes_that_take_the_largest_tiles(T, K, N, lens, dtype):
     check(x, w, b, dy, edges(T, lens))
 
 
+@pytest.mark.parametrize("K,N", [(2048, 24), (40, 2048)])
+def test_rows_of_more_than_2_to_the_31_elements(K, N):
+    """x and dx, or y and dy, beyond 2^31 elements: the last groups, whose rows lie behind that, and their gradients"""
+    from uemda_amd.grouped import grouped_linear
+    T = 2 ** 31 // 2048 + 9000
+    o = [100, T - 7000, T - 4000, T - 1000]
+    gen = torch.Generator(device="cuda").manual_seed(K)
+    x, dy = (torch.randn(T, n, generator=gen, device="cuda", dtype=torch.bfloat16) for n in (K, N))
+    w, b = torch.randn(3, N, K, generator=gen, device="cuda", dtype=torch.bfloat16), torch.randn(3, N, generator=gen, device="cuda", dtype=torch.bfloat16)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = grouped_linear(x, w, torch.tensor(o, device="cuda"), b)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        at = T - 8000                                                          # the end of the first group, the others, and the tail
+        (ry, ay), (rdx, ax), (rdw, aw), (rdb, ab) = reference(x[at:], w, b, dy[at:], [0, 1000, 4000, 7000])
+        close(y[at:], ry, ay, K + 1, "y")
+        close(dx[at:], rdx, ax, N, "dx")
+        close(dw[1:], rdw[1:], aw[1:], 3000, "dw")
+        close(db[1:], rdb[1:], ab[1:], 3000, "db")
+        assert not y[:100].any() and not dx[:100].any()
+        want, mag = 0, 0
+        for s in range(o[0], o[1], 2 ** 17):                                   # the first group's gradients: nearly all of the rows
+            e = min(o[1], s + 2 ** 17)
+            want = want + dy[s:e].double().sum(0)
+            mag = mag + dy[s:e].double().abs().sum(0)
+        close(db[0], want, mag, o[1] - o[0], "db of the long group")
+
+
 def test_master_weights_int64_offsets_and_no_bias():
     o = edges(200, [60, 0, 100], 7)
     x, w, b, dy = data(200, 3, 48, 56, torch.bfloat16, 1, wdtype=torch.float32, bdtype=torch.float32)

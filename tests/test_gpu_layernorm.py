@@ -95,6 +95,35 @@ def test_optional_and_16_bit_parameters(dtype, have):
     check(x, w if "w" in have else None, b if "b" in have else None, dy)
 
 
+@pytest.mark.parametrize("c", [2048, 777, 120])
+def test_maps_of_more_than_2_to_the_31_elements(c):
+    """every row's y and dx, and the parameter gradients over all of them, checked a slice at a time"""
+    from uemda_amd.norm import layer_norm
+    rows, part = (2 ** 31 + 2 ** 24) // c, 2 ** 27 // c
+    gen = torch.Generator(device="cuda").manual_seed(c)
+    x = torch.randn(rows, c, generator=gen, device="cuda", dtype=torch.bfloat16).requires_grad_()
+    dy = torch.randn(rows, c, generator=gen, device="cuda", dtype=torch.bfloat16)
+    w = torch.randn(c, generator=gen, device="cuda").requires_grad_()
+    b = torch.randn(c, generator=gen, device="cuda").requires_grad_()
+    y = layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    sums = [torch.zeros(c, dtype=torch.float64, device="cuda") for _ in range(4)]
+    Dr = rows / 64 + 64
+    with torch.no_grad():
+        for at in list(range(0, rows, part)):
+            s = slice(at, min(rows, at + part))
+            r = reference(x[s], w, b, dy[s], 1e-5)
+            ey, edx, edw, edb = bounds(x[s], dy[s], b, r)
+            close(y[s], r[0], ey, "y")
+            close(dx[s], r[1], edx, "dx")
+            mag = dy[s].double().abs().sum(0), (dy[s].double() * r[4]).abs().sum(0)
+            for t, v in zip(sums, (r[2], edw + U * Dr * mag[1], r[3], edb + U * Dr * mag[0])):
+                t += v
+            del r, ey, edx
+    close(dw, sums[0], sums[1], "dw")
+    close(db, sums[2], sums[3], "db")
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_a_mean_far_from_zero_keeps_its_variance(dtype):
     check(*data(40, 640, dtype, 5, offset=100.0))
