@@ -12,8 +12,8 @@
 // 16-byte chunks on the source address so that a read covers all banks.  Buffer descriptors that end with the group's last row (and
 // offsets beyond them for columns past the end) supply the zeros of every ragged edge: no row of another group is ever read.
 // Products are exact in the fp32 accumulators (bf16) or fp32 MFMA (fp32); bf16 results are rounded once.
-// Measured, bf16, 65536 x 2048 -> 2048 in 32 ragged groups, us: forward 530 - 565, data gradient 495 - 516, weight gradient with db 483 - 510
-// (550 GFLOP each: 0.97 - 1.14 PFLOP/s; a dense library product of the size takes 467): the clock falls to 1.7 GHz under the products, what
+// Measured, bf16, 65536 x 2048 -> 2048 in 32 ragged groups, us: forward 505 - 545, data gradient 495 - 516, weight gradient with db 483 - 510
+// (550 GFLOP each: 1.01 - 1.14 PFLOP/s; in groups of 2048 rows 470 = 1.17, a dense library product of the size 467): the clock falls to 1.7 GHz under the products, what
 // is left is a tile's start and end.  fp32, 65536 x 2048 -> 2048 in 8 groups: 3.9 ms = 142 TFLOP/s of the 151 a dense product reaches.
 //
 // Nothing is read on the host: a block finds its tiles by prefix sums over the offsets, 64 groups to a wave, kept in registers.  Offsets are clamped to [0, T] and to the largest one in front of them, so that any
@@ -331,6 +331,8 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     constexpr bool PP = NW == 8, AKS = FORM == WGRAD, BKS = FORM != FWD;
     using LA = Loader<T, AKS, BM, NW>;
     using LB = Loader<T, BKS, BN, NW>;
+    constexpr bool SPLIT = PP && !AKS && !BKS && LB::IPW % 2 == 0;       // both operands KC: b's pairs leave in halves
+    constexpr int FLIGHT_EVEN = 2 * LA::IPW + LB::IPW;                         // SPLIT, in front of an even stage
     constexpr int FLIGHT = LA::IPW * (AKS ? 3 : 2) + LB::IPW * (BKS ? 3 : 2);
     constexpr int ROWB = NT * 64, CPR = ROWB / 16;                             // bf16 results: bytes and 16-byte chunks of a wave's row
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -399,30 +401,34 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
         if (AKS) { pa += BK * p.lda; arem -= BK; }
         qa += two ? 2 : 1;
     };
-    auto issue_b = [&](char* __restrict__ fill0, char* __restrict__ fill1, const bool two) {
+    auto issue_b = [&](char* __restrict__ fill0, char* __restrict__ fill1, const bool two, const int first, const int end) {
         const i32x4 r0_ = desc(pb, brem, p.ldb, bcols, BKS);
         if (BKS || (PP && (qb + (two ? 2 : 1)) * BK <= red)) {
 #pragma unroll
-            for (int j = 0; j < LB::IPW; ++j) {
+            for (int j = first; j < end; ++j) {
                 lb.issue_whole(j, r0_, fill0 + BM * 64, wave, qb);
                 if (two) lb.issue_whole(j, r0_, fill1 + BM * 64, wave, qb + 1);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < LB::IPW; ++j) {
+            for (int j = first; j < end; ++j) {
                 lb.issue(j, r0_, fill0 + BM * 64, wave, qb, red);
                 if (two) lb.issue(j, r0_, fill1 + BM * 64, wave, qb + 1, red);
             }
         }
+        if (end < LB::IPW) return;
         if (BKS) { pb += BK * p.ldb; brem -= BK; }
         qb += two ? 2 : 1;
     };
-    // in stage t: a KC operand's stages t + 3 and t + 4 if t is odd, a KS operand's stage t + 4
-    auto issue = [&](char* __restrict__ fill3, char* __restrict__ fill4, const bool odd) {
+    // in stage t: a KC operand's stages t + 3 and t + 4 if t is odd (SPLIT: of b half their pieces, the other half in the stage behind; with all of
+    // both operands in the odd stages 65536 x 2048 -> 2048 in 32 groups took 500 us, so 470), a KS operand's stage t + 4
+    auto issue = [&](char* __restrict__ fill2, char* __restrict__ fill3, char* __restrict__ fill4, const bool odd) {
         if (AKS) issue_a(fill4, fill4, false);
         else if (odd) issue_a(fill3, fill4, true);
-        if (BKS) issue_b(fill4, fill4, false);
-        else if (odd) issue_b(fill3, fill4, true);
+        if (BKS) issue_b(fill4, fill4, false, 0, LB::IPW);
+        else if (!SPLIT) { if (odd) issue_b(fill3, fill4, true, 0, LB::IPW); }
+        else if (odd) issue_b(fill3, fill4, true, 0, LB::IPW / 2);
+        else issue_b(fill2, fill3, true, LB::IPW / 2, LB::IPW);
     };
     f32x16 acc[MT][NT];
 #pragma unroll
@@ -439,7 +445,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     Frag<T, BKS, BN> fb[2][NT];
     // one function with the stages being refilled and the stage being read as __restrict__ pointers: that is what tells the compiler that
     // the reads do not depend on the LDS-DMA in flight (it would wait for all of it in front of the first read)
-    auto stage = [&](char* __restrict__ fill3, char* __restrict__ fill4, const char* __restrict__ use, const bool odd) {
+    auto stage = [&](char* __restrict__ fill2, char* __restrict__ fill3, char* __restrict__ fill4, const char* __restrict__ use, const bool odd) {
         auto fetch = [&](const int ks) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) fa[ks][i].load(use, wm + i * 32, ks, lane);
@@ -459,13 +465,15 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
                 if (i == wave % WGN) colsum = add_of(fa[1][i], add_of(fa[0][i], colsum, T{}), T{});
         };
         // In front of stage t (PP: in stage t - 1, behind its sends) the pieces of stage t have to have landed.  Newer than the last of them
-        // are, of a KS operand, three stages' pieces and, of a KC operand, those of the pair behind its own (and, t even, its partner's last).
+        // are, of a KS operand, three stages' pieces and, of a KC operand, those of the pair behind its own (and, t even, its partner's last;
+        // SPLIT, t even: what one odd stage sends; t odd: that and the halves of the even stage behind it).
         if (PP) {
             fetch(0);
             fetch(1);
             __builtin_amdgcn_sched_barrier(0);                                 // the reads first: the sends' addresses are made in their shadow
-            issue(fill3, fill4, odd);
-            gg_wait<FLIGHT>();
+            issue(fill2, fill3, fill4, odd);
+            if (SPLIT && odd) gg_wait<FLIGHT_EVEN>();
+            else gg_wait<FLIGHT>();
             if (FORM == WGRAD) add_up();
             gg_barrier();
             __builtin_amdgcn_s_setprio(1);
@@ -477,7 +485,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
         } else {
             gg_wait<FLIGHT>();
             gg_barrier();
-            issue(fill3, fill4, odd);
+            issue(fill2, fill3, fill4, odd);
             fetch(0);
             fetch(1);
             multiply(0);
@@ -492,22 +500,23 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
             char* const f0 = smem + t * SB;
             char* const f1 = f0 + SB;
             if (!AKS) issue_a(f0, f1, true);
-            if (!BKS) issue_b(f0, f1, true);
+            if (!BKS) issue_b(f0, f1, true, 0, SPLIT && t == 2 ? LB::IPW / 2 : LB::IPW);
             if (AKS) issue_a(f0, f0, false);
-            if (BKS) issue_b(f0, f0, false);
+            if (BKS) issue_b(f0, f0, false, 0, LB::IPW);
             if (AKS) issue_a(f1, f1, false);
-            if (BKS) issue_b(f1, f1, false);
+            if (BKS) issue_b(f1, f1, false, 0, LB::IPW);
         }
         if (PP) {
-            gg_wait<FLIGHT>();
+            if (SPLIT) gg_wait<FLIGHT_EVEN>();
+            else gg_wait<FLIGHT>();
             gg_barrier();
             if (wave >= NW / 2) gg_barrier();
         }
         int u = 0;                                                             // stage t's place in the ring
         auto place = [](int k) { return (k >= NST ? k - NST : k) * SB; };
         for (int t = 0; t < steps; t += 2) {                                   // an odd number of stages: the last one multiplies zeros
-            stage(smem + place(u + 3), smem + place(u + 4), smem + u * SB, false);
-            stage(smem + place(u + 4), smem + u * SB, smem + place(u + 1), true);
+            stage(smem + place(u + 2), smem + place(u + 3), smem + place(u + 4), smem + u * SB, false);
+            stage(smem + place(u + 3), smem + place(u + 4), smem + u * SB, smem + place(u + 1), true);
             u = u + 2 >= NST ? u + 2 - NST : u + 2;
         }
         if (PP && wave < NW / 2) gg_barrier();
