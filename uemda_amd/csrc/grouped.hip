@@ -301,11 +301,21 @@ __device__ __forceinline__ void gg_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// rows of no group, shared out over the grid: zeros
+// Rows of no group: zeros.  Shared out over the blocks without one of the n items (there are as a rule as many as such rows make tiles; they come
+// last, when CUs run out of items: 32768 rows x 512, half of them of no group, 21.5 -> 19.4 us; a fifth, x 512 of 2048, 70.5 -> 68.5; at worst
+// 65536 x 1024, half of them, 80.3 -> 82.5), or over all if there is none.
 template <int NTH>
-__device__ __forceinline__ void zero_rows(const GgP& p, const Groups<false>& groups, int width) {
-    const int head = groups.first, zeros = head + p.T - groups.last;
-    for (int z = blockIdx.x; z < zeros; z += gridDim.x) {
+__device__ __forceinline__ void zero_rows(const GgP& p, const Groups<false>& groups, int width, int n) {
+    const int head = groups.first, zeros = head + p.T - groups.last, free = (int)gridDim.x - n;
+    int z = blockIdx.x, step = gridDim.x;
+    if (free > 0) {
+        const int x = blockIdx.x & 7, i = blockIdx.x >> 3, per = n >> 3, rem = n & 7;
+        const int late = i - per - (x < rem ? 1 : 0);                          // its place among its XCD's blocks without an item
+        if (late < 0) return;
+        z = x * ((int)(gridDim.x >> 3) - per) - (x < rem ? x : rem) + late;
+        step = free;
+    }
+    for (; z < zeros; z += step) {
         const int64_t at = (int64_t)(z < head ? z : groups.last + z - head) * p.ldo;
         if (p.vec) {
             const int n = p.out16 ? 8 : 4;
@@ -317,7 +327,7 @@ __device__ __forceinline__ void zero_rows(const GgP& p, const Groups<false>& gro
         }
     }
 }
-template <int NTH> __device__ __forceinline__ void zero_rows(const GgP&, const Groups<true>&, int) {}
+template <int NTH> __device__ __forceinline__ void zero_rows(const GgP&, const Groups<true>&, int, int) {}
 
 // One tile a block.  Five stages: while stage t is computed on, a KS operand's pieces of stage t + 4 leave, a KC operand's of stages t + 3 and
 // t + 4 together if t is odd -- the two halves of every 128-byte line one after the other, or the line travels from L2 twice (65536 x 2048 ->
@@ -344,7 +354,7 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     Groups<FORM == WGRAD> groups;
     groups.init(p, bm, lane);
 
-    if (FORM != WGRAD) zero_rows<64 * NW>(p, groups, width);
+    if (FORM != WGRAD) zero_rows<64 * NW>(p, groups, width, groups.total * ct);
     const int item = FORM == WGRAD ? ((int)blockIdx.x < (groups.total + groups.rests) * ct * rt ? (int)blockIdx.x : -1) : xcd_item(groups.total * ct * rt);
     if (item < 0) return;
 
@@ -616,8 +626,8 @@ __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Groups<false> groups;
     groups.init(p, 32, lane);
-    zero_rows<1024>(p, groups, p.N);
     const int ct = (p.N + 31) / 32, item = xcd_item(groups.total * ct);
+    zero_rows<1024>(p, groups, p.N, groups.total * ct);
     if (item < 0) return;
     const Tile tl = groups.find(p, 32, lane, item / ct);
     const int c0 = (item % ct) * 32, r0 = tl.row0 + tl.tile * 32, rows = min(32, tl.rows - tl.tile * 32);
