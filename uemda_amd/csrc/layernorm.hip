@@ -415,18 +415,42 @@ __global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __r
     }
 }
 
-constexpr int LN_BWD_BLOCKS = 1024;            // most partial sums the backward leaves
+// most blocks the backward of so many rows takes: each leaves its partial sums, which are to stay a fraction of what its rows read and write
+// (2000 x 2048 bf16: 256 blocks 19 us, 768 22, 1536 33)
+int64_t bwd_blocks(int64_t rows) {
+    const int64_t n = uem_cdiv(rows < 256 ? rows : rows < 2048 ? 256 : rows / 8, 8) * 8;
+    return n > 2048 ? 2048 : n;
+}
+// blocks of a kernel that a CU holds at once (registers): asked for once
+template <typename K> int resident(K kernel) {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, 0) != hipSuccess || n < 1) n = 4;
+    return n > 8 ? 8 : n;
+}
 
 template <typename T, int LPR, int NV, int MODE>
 int go(const LnP& p, bool bwd, hipStream_t st) {
-    // Measured, us (fp32 32768 x 2048 | bf16 524288 x 256 | bf16 65536 x 777; a plain copy of the map takes 100 | 101 | 29):
-    //   forward, grid of at most 1024 / 4096 / 16384 blocks: 97 / 99 / 91 | 103 / 108 / 100 | 42 / 42 / 69; two rows in flight a team gain
-    //   nothing (92 | 100 | 56).  So: no cap worth the name on the 16-byte grid, 1024 blocks where a team's parameters cost more to load.
-    //   backward, 512 / 1024 / 2048 blocks: one row 146 / 165 / 172 | 259 / 168 / 184 | 126 / 134 / 124, two rows 154 / 169 / 179 |
-    //   235 / 157 / 162 | 125 / 133 / 150: every block costs its partial sums; two rows only where a team is part of a wave.
+    // Grids that the chip holds at once: another block of a CU's would run behind the others, and where rows cost instructions (bf16, or rows
+    // that are not aligned) fewer leave them uncovered.  Measured, us (2^26 elements unless said), backward, 512 / 768 / 1024 / 1536 / 2048 blocks:
+    //   bf16 of 2^27: 256 columns (4 a CU) 233 / 177 / 152 / 186 / 159, 2048 (6) 267 / 207 / 177 / 162 / 199; bf16 777 (3) 165 / 126 / 176 / 136 / 153,
+    //   33 (8) 1252 / 854 / 657 / 469 / 374; fp32 1001 204 / 155 / 163 / 175 / 179.
+    // Aligned fp32 rows are so few instructions a byte that two blocks a CU, three where a lane holds one access, do best: 2^27 elements
+    //   in 256 columns 290 / 293 / 301 / 323 / 330, 2048 289 / 294 / 323 / 326 / 324, 1024 312 / 287 / 296 / 324 / 324.
+    // forward, 1024 / 1536 / 2048 / 16384: bf16 2049 columns (6) 81 / 65 / 82 / 104, 4096 (6) 52 / 44 / 53 / 61; fp32 7 (8) 276 / 218 / 190 / 194.
+    //   Aligned rows of up to a wave, and fp32 ones, are fastest with a block for as few rows as there are: 256 columns bf16 48 / 46 / 46 / 44,
+    //   fp32 98 / 103 / 110 / 98 (91 with 65536 blocks).
+    // Two rows in flight a team gain where a team is part of a wave, backward alone: 168 against 157.
     constexpr int UB = LPR < 64 ? 2 : 1, TEAMS = 256 / LPR;
-    int64_t nb = uem_cdiv(p.rows, TEAMS * (bwd ? UB : 1));
-    const int64_t most = bwd ? (LPR > 64 || MODE == 1 ? LN_BWD_BLOCKS / 2 : LN_BWD_BLOCKS) : MODE == 0 ? 16384 : 1024;
+    constexpr bool f32 = sizeof(T) == 4;
+    static const int fit = resident(layernorm_fwd_kernel<T, LPR, NV, MODE>), fit_bwd = resident(layernorm_bwd_kernel<T, LPR, NV, MODE, UB>);
+    int64_t nb = uem_cdiv(p.rows, TEAMS * (bwd ? UB : 1)), most;
+    if (bwd) {
+        const int few = MODE == 1 || (LPR > 64 && NV == 1) ? 3 : 2;
+        most = 256 * (f32 && MODE != 2 && fit_bwd > few ? few : fit_bwd);
+        if (most > bwd_blocks(p.rows)) most = bwd_blocks(p.rows);
+    } else {
+        most = MODE == 0 && (f32 || LPR <= 64) ? 16384 : 256 * fit;
+    }
     if (nb > most) nb = most;
     if (MODE == 1) nb = uem_cdiv(nb, 8) * 8;                                   // teams % period == 0 (period <= 8)
     if (bwd) layernorm_bwd_kernel<T, LPR, NV, MODE, UB><<<(int)nb, 256, 0, st>>>(p);
@@ -481,8 +505,9 @@ int run(LnP p, bool bwd, hipStream_t st) {
 }  // namespace
 
 extern "C" int64_t uem_layernorm_workspace_floats(int64_t rows, int C) {
-    const int64_t most = C > 8192 ? 64 : LN_BWD_BLOCKS;                        // longer rows: the pass over columns
-    return (rows < most ? uem_cdiv(rows, 8) * 8 : most) * 2 * (int64_t)C;
+    int64_t n = bwd_blocks(rows);
+    if (C > 8192 && n > 64) n = 64;                                            // longer rows: the pass over columns
+    return n * 2 * (int64_t)C;
 }
 extern "C" int uem_layernorm_fwd(const void* x, int64_t x_ld, const void* gamma, const void* beta, void* y, float* mean, float* rstd,
                                  int64_t rows, int C, float eps, int flags, void* stream) {
