@@ -79,7 +79,7 @@ def check(x, w, b, dy, eps=1e-5):
 
 SIZES = [(1, 1), (3, 1), (1, 2), (5, 8), (7, 9), (1000, 7), (33, 64), (17, 100), (130, 128), (129, 256), (64, 257), (66, 260), (300, 777),
          (41, 1001), (1031, 96), (12, 1024), (9, 1026), (33, 2048), (17, 2049), (9, 4100), (7, 5000), (3, 8192), (2, 8191), (2, 8200), (2, 20001),
-         (1, 2048), (9000, 48), (5000, 513)]
+         (1, 2048), (9000, 48), (5000, 513), (100, 33), (40001, 33), (1000, 50), (3001, 17), (20, 13), (5000, 67), (129, 131), (77, 203), (5001, 255)]
 
 
 @pytest.mark.parametrize("rows,c", SIZES)
@@ -95,7 +95,7 @@ def test_optional_and_16_bit_parameters(dtype, have):
     check(x, w if "w" in have else None, b if "b" in have else None, dy)
 
 
-@pytest.mark.parametrize("c", [2048, 777, 120])
+@pytest.mark.parametrize("c", [2048, 777, 120, 33])
 def test_maps_of_more_than_2_to_the_31_elements(c):
     """every row's y and dx, and the parameter gradients over all of them, checked a slice at a time"""
     from uemda_amd.norm import layer_norm

@@ -63,7 +63,7 @@ struct LnP {
 //   MODE 1: dense rows of any length: 16-byte accesses on the allocation's own boundaries, shift = the row's start modulo W; the row's
 //           first and last access go element by element.  Rows r and r + period start alike: a team walks rows of ONE start (r mod
 //           period), so that its columns stay fixed
-//   MODE 2: element by element (short rows that are not aligned)
+//   MODE 2: element by element (short rows that are not aligned, where that is faster or the tensor is not dense)
 template <typename T, int LPR, int NV, int MODE>
 struct Row {
     static constexpr int W = MODE == 2 ? 1 : Vec<T>::N;
@@ -229,7 +229,13 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
     __shared__ float join[2][CAP];
     int flip = 0;
     const int lane = threadIdx.x % LPR;
-    const int64_t team = (int64_t)blockIdx.x * TEAMS + threadIdx.x / LPR, teams = (int64_t)gridDim.x * TEAMS;
+    const int64_t teams = (int64_t)gridDim.x * TEAMS;
+    int64_t team = (int64_t)blockIdx.x * TEAMS + threadIdx.x / LPR, block0 = (int64_t)blockIdx.x * TEAMS;      // first row of the team, of the block
+    if (MODE == 1 && LPR < 64) {                                               // the teams of a wave on rows that start alike: they add up their columns
+        const int w = blockIdx.x * 4 + (threadIdx.x >> 6), w0 = blockIdx.x * 4, per = p.period * (64 / LPR);
+        team = (int64_t)(w / p.period) * per + (threadIdx.x & 63) / LPR * p.period + w % p.period;
+        block0 = (int64_t)(w0 / p.period) * per + w0 % p.period;
+    }
     const int shift = MODE == 1 ? (int)(((team % p.period) * p.C) & (W - 1)) : 0;
     const float inv = 1.f / (float)p.C;
     float ga[NV][W], aw[NV][W], ab[NV][W];
@@ -238,7 +244,7 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < W; ++e) aw[i][e] = ab[i][e] = 0.f;
-    for (int64_t base = (int64_t)blockIdx.x * TEAMS, r = team; base < p.rows; base += teams * U, r += teams * U) {
+    for (int64_t base = block0, r = team; base < p.rows; base += teams * U, r += teams * U) {
         float v[U][NV][W], g[U][NV][W], mean[U], rstd[U], s[2 * U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -442,22 +448,34 @@ int go(const LnP& p, bool bwd, hipStream_t st) {
     // Two rows in flight a team gain where a team is part of a wave, backward alone: 168 against 157.
     constexpr int UB = LPR < 64 ? 2 : 1, TEAMS = 256 / LPR;
     constexpr bool f32 = sizeof(T) == 4;
-    static const int fit = resident(layernorm_fwd_kernel<T, LPR, NV, MODE>), fit_bwd = resident(layernorm_bwd_kernel<T, LPR, NV, MODE, UB>);
-    int64_t nb = uem_cdiv(p.rows, TEAMS * (bwd ? UB : 1)), most;
-    if (bwd) {
-        const int few = MODE == 1 || (LPR > 64 && NV == 1) ? 3 : 2;
-        most = 256 * (f32 && MODE != 2 && fit_bwd > few ? few : fit_bwd);
-        if (most > bwd_blocks(p.rows)) most = bwd_blocks(p.rows);
-    } else {
-        most = MODE == 0 && (f32 || LPR <= 64) ? 16384 : 256 * fit;
+    auto grid = [&](int rows, int64_t most) {
+        int64_t n = uem_cdiv(p.rows, rows);
+        if (n > most) n = most;
+        return (int)(MODE == 1 ? uem_cdiv(n, 8) * 8 : n);                      // teams % period == 0 (period <= 8)
+    };
+    if (!bwd) {
+        static const int fit = resident(layernorm_fwd_kernel<T, LPR, NV, MODE>);
+        const int nb = grid(TEAMS, MODE == 0 && (f32 || LPR <= 64) ? 16384 : 256 * fit);
+        layernorm_fwd_kernel<T, LPR, NV, MODE><<<nb, 256, 0, st>>>(p);
+        return nb;
     }
-    if (nb > most) nb = most;
-    if (MODE == 1) nb = uem_cdiv(nb, 8) * 8;                                   // teams % period == 0 (period <= 8)
-    if (bwd) layernorm_bwd_kernel<T, LPR, NV, MODE, UB><<<(int)nb, 256, 0, st>>>(p);
-    else layernorm_fwd_kernel<T, LPR, NV, MODE><<<(int)nb, 256, 0, st>>>(p);
-    return bwd && nb == 1 ? 0 : (int)nb;                                       // 0: no partial sums left
+    if constexpr (!(f32 && MODE == 1 && LPR < 64)) {                           // (such rows go forward only: run)
+        static const int fit = resident(layernorm_bwd_kernel<T, LPR, NV, MODE, UB>);
+        const int few = MODE == 1 || (LPR > 64 && NV == 1) ? 3 : 2;
+        const int64_t most = 256 * (f32 && MODE != 2 && fit > few ? few : fit), leave = bwd_blocks(p.rows);
+        const int nb = grid(TEAMS * UB, most < leave ? most : leave);
+        layernorm_bwd_kernel<T, LPR, NV, MODE, UB><<<nb, 256, 0, st>>>(p);
+        return nb == 1 ? 0 : nb;                                               // 0: no partial sums left
+    }
+    return 0;
 }
 
+// dense rows of C elements r and r + period start alike modulo w elements
+int period_of(int C, int w) {
+    int n = w;
+    while (n > 1 && ((int64_t)(n / 2) * C) % w == 0) n /= 2;
+    return n;
+}
 template <typename T>
 int run(LnP p, bool bwd, hipStream_t st) {
     constexpr int W = Vec<T>::N;
@@ -478,6 +496,16 @@ int run(LnP p, bool bwd, hipStream_t st) {
         if (v <= 512) return go<T, 256, 2, 0>(p, bwd, st);
         if (v <= 1024) return go<T, 256, 4, 0>(p, bwd, st);
         if (W == 4 && v <= 2048) return go<T, 256, W == 4 ? 8 : 4, 0>(p, bwd, st);
+    } else if (base16 && dense && (W == 8 ? p.C > (bwd ? 16 : 8) && p.C <= 256 : !bwd && p.C > 8 && p.C <= 64)) {
+        // Short rows in whole accesses, against element by element, us at 2^26 elements: bf16 forward 9 columns 450 / 274, 33 273 / 129, 100 158 / 80,
+        // 255 133 / 93; backward 9 597 / 601, 20 288 / 262, 33 379 / 221, 100 225 / 130, 255 170 / 128.  fp32, twice the bytes an element: forward
+        // 9 465 / 288, 33 278 / 195, 67 170 / 169, 131 130 / 156; backward 9 337 / 511, 33 249 / 277, 131 186 / 221.
+        const int v = (p.C + W - 1 + W - 1) / W;                               // accesses of the worst start
+        p.period = period_of(p.C, W);
+        if (v <= 8) return go<T, 8, 1, 1>(p, bwd, st);
+        if (v <= 16) return go<T, 16, 1, 1>(p, bwd, st);
+        if (v <= 32) return go<T, 32, 1, 1>(p, bwd, st);
+        if (W == 8) return go<T, 64, W == 8 ? 1 : 2, 1>(p, bwd, st);
     } else if (p.C <= 256) {
         if (p.C <= 8) return go<T, 8, 1, 2>(p, bwd, st);
         if (p.C <= 32) return go<T, 32, 1, 2>(p, bwd, st);
@@ -485,8 +513,7 @@ int run(LnP p, bool bwd, hipStream_t st) {
         return go<T, 64, 4, 2>(p, bwd, st);
     } else if (base16 && dense) {
         const int v = (p.C + W - 1 + W - 1) / W;                               // accesses of the worst start
-        p.period = W;
-        while (p.period > 1 && ((int64_t)(p.period / 2) * p.C) % W == 0) p.period /= 2;
+        p.period = period_of(p.C, W);
         if (v <= 128) return go<T, 64, 2, 1>(p, bwd, st);
         if (v <= 256) return go<T, 256, 1, 1>(p, bwd, st);
         if (v <= 512) return go<T, 256, 2, 1>(p, bwd, st);
