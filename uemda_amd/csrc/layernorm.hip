@@ -2,7 +2,7 @@
 //   y = (x - mean) * rstd * gamma + beta,   mean = sum x / C,   rstd = 1 / sqrt(sum (x - mean)^2 / C + eps)
 //   dx = rstd * (g - mean(g) - xhat * mean(g * xhat)),  g = dy * gamma,  xhat = (x - mean) * rstd
 //   dgamma = sum_rows dy * xhat,   dbeta = sum_rows dy
-// Bound by HBM: 2 row reads/writes forward, 3 backward, ~8 / ~14 flops an element.  A row is read ONCE: a team of lanes keeps it in
+// Bound by HBM: 2 row reads/writes forward, 3 backward, ~8 / ~14 flops an element (32768 x 2048 fp32: 87 us = 6.2 TB/s, 151 = 5.3).  A row is read ONCE: a team of lanes keeps it in
 // registers between the two sums of the statistics (the squares are summed about the mean, in 32 bits) and the output, so a row costs
 // its bytes and two reductions by lane exchange.  Backward, a team walks rows with its columns fixed, so dgamma / dbeta accumulate in
 // registers too; a block's teams are joined in LDS and the blocks' partial sums by a second small launch, in a fixed order: the result
@@ -138,9 +138,9 @@ __device__ __forceinline__ void team_sums(float (&v)[K], float* red, int& flip) 
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         if (LPR >= 64) { v[k] = wave_sum_dpp(v[k]); continue; }
-        v[k] += dpp_take0<0xB1, 0xF>(v[k]);
-        v[k] += dpp_take0<0x4E, 0xF>(v[k]);
-        v[k] += dpp_take0<0x141, 0xF>(v[k]);
+        if (LPR >= 2) v[k] += dpp_take0<0xB1, 0xF>(v[k]);
+        if (LPR >= 4) v[k] += dpp_take0<0x4E, 0xF>(v[k]);
+        if (LPR >= 8) v[k] += dpp_take0<0x141, 0xF>(v[k]);
         if (LPR >= 16) v[k] += dpp_take0<0x140, 0xF>(v[k]);
         if (LPR >= 32) v[k] += __shfl_xor(v[k], 16, 64);
     }
@@ -483,10 +483,13 @@ int run(LnP p, bool bwd, hipStream_t st) {
     const bool base16 = (bases & 15) == 0;
     const bool dense = p.x_ld == p.C && (!bwd || p.dy_ld == p.C);
     p.period = 1;
-    // Lanes per row: one wave while a lane holds at most 16 elements (8 in bf16's wide accesses), a block of four above -- backward keeps
+    // Lanes per row: as many as it has accesses; one wave while a lane holds at most 16 elements (8 in bf16's wide accesses), a block of four above -- backward keeps
     // five values an element in registers (x, g, gamma and the two parameter gradients), 32 elements a lane would leave two waves a SIMD
     if (base16 && p.C % W == 0 && p.x_ld % W == 0 && (!bwd || p.dy_ld % W == 0)) {
         const int v = p.C / W;
+        if (v <= 1) return go<T, 1, 1, 0>(p, bwd, st);
+        if (v <= 2) return go<T, 2, 1, 0>(p, bwd, st);
+        if (v <= 4) return go<T, 4, 1, 0>(p, bwd, st);
         if (v <= 8) return go<T, 8, 1, 0>(p, bwd, st);
         if (v <= 16) return go<T, 16, 1, 0>(p, bwd, st);
         if (v <= 32) return go<T, 32, 1, 0>(p, bwd, st);
@@ -496,17 +499,20 @@ int run(LnP p, bool bwd, hipStream_t st) {
         if (v <= 512) return go<T, 256, 2, 0>(p, bwd, st);
         if (v <= 1024) return go<T, 256, 4, 0>(p, bwd, st);
         if (W == 4 && v <= 2048) return go<T, 256, W == 4 ? 8 : 4, 0>(p, bwd, st);
-    } else if (base16 && dense && (W == 8 ? p.C > (bwd ? 16 : 8) && p.C <= 256 : !bwd && p.C > 8 && p.C <= 64)) {
-        // Short rows in whole accesses, against element by element, us at 2^26 elements: bf16 forward 9 columns 450 / 274, 33 273 / 129, 100 158 / 80,
-        // 255 133 / 93; backward 9 597 / 601, 20 288 / 262, 33 379 / 221, 100 225 / 130, 255 170 / 128.  fp32, twice the bytes an element: forward
-        // 9 465 / 288, 33 278 / 195, 67 170 / 169, 131 130 / 156; backward 9 337 / 511, 33 249 / 277, 131 186 / 221.
+    } else if (base16 && dense && p.C > 8 && (W == 8 ? p.C <= 256 : !bwd && p.C <= 64)) {
+        // Short rows in whole accesses, against element by element, us at 2^26 elements: bf16 forward 33 columns 273 / 129, 100 158 / 80, 255 133 / 93,
+        // backward 33 379 / 221, 100 225 / 130, 255 170 / 128; at 2^25 forward 7 82 / 78, backward 7 110 / 214, 9 298 / 212, 13 214 / 157.  fp32, twice the
+        // bytes an element: forward 33 278 / 195, 67 170 / 169, 131 130 / 156; backward 33 249 / 277, 131 186 / 221, at 2^25 9 172 / 227.
         const int v = (p.C + W - 1 + W - 1) / W;                               // accesses of the worst start
         p.period = period_of(p.C, W);
+        if (v <= 2) return go<T, 2, 1, 1>(p, bwd, st);
+        if (v <= 4) return go<T, 4, 1, 1>(p, bwd, st);
         if (v <= 8) return go<T, 8, 1, 1>(p, bwd, st);
         if (v <= 16) return go<T, 16, 1, 1>(p, bwd, st);
         if (v <= 32) return go<T, 32, 1, 1>(p, bwd, st);
         if (W == 8) return go<T, 64, W == 8 ? 1 : 2, 1>(p, bwd, st);
     } else if (p.C <= 256) {
+        if (p.C <= 4) return go<T, 4, 1, 2>(p, bwd, st);
         if (p.C <= 8) return go<T, 8, 1, 2>(p, bwd, st);
         if (p.C <= 32) return go<T, 32, 1, 2>(p, bwd, st);
         if (p.C <= 64) return go<T, 64, 1, 2>(p, bwd, st);
