@@ -95,6 +95,8 @@ SHAPES = [
     (2600, 264, 272, [1300, 0, 1290], 5),
     (6000, 320, 320, [5800, 30, 100], 0),            # one group of several chunks in the weight gradient
     (4100, 40, 48, [4100], 0),
+    (20000, 24, 16, [19000, 900], 3),                # and of many
+    (20001, 23, 17, [20000], 1),
     (3500, 40, 136, [3] * 40 + [900] + [0] * 30 + [1100] + [5] * 20 + [256, 512, 300], 4),     # chunks and rests on both sides of lane 64
 ]
 

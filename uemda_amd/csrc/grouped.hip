@@ -673,44 +673,61 @@ __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
 // the sum of n values `step` apart, in their order, four of them on the way at a time
 template <typename V> __device__ __forceinline__ V sum_in_order(const V* p, int64_t step, int n) {
     V v = *p;
-    int c = 1;
-    for (; c + 3 < n; c += 4) {
+    for (int c = 1; c < n; c += 4) {
         V u[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) u[k] = p[(c + k) * step];
+        for (int k = 0; k < 4; ++k) u[k] = c + k < n ? p[(c + k) * step] : V{};
 #pragma unroll
         for (int k = 0; k < 4; ++k) v += u[k];
     }
-    for (; c < n; ++c) v += p[c * step];
     return v;
 }
-// dW and db of the groups of several chunks = their partial sums, added in row order.  blockIdx.y: which of those groups
+// store(i, sum of src[i], src[i + step] ... n of them) for i < count, by the block `block` of `blocks`.  Many chunks are shared out over 4 or 16
+// slices of the block, whose sums are added in order (65536 rows, 64 -> 32 in one group, 256 chunks: 40 us by one thread an
+// element, 5 so)
+template <typename V, typename S> __device__ __forceinline__ void join_sums(const V* src, int64_t count, int64_t step, int n, int block, int blocks, V* red, S store) {
+    const int slices = n > 64 ? 16 : n > 16 ? 4 : 1, lanes = 256 / slices, l = threadIdx.x % lanes, sl = threadIdx.x / lanes;
+    const int c0 = (int)((int64_t)n * sl / slices), c1 = (int)((int64_t)n * (sl + 1) / slices);
+    for (int64_t base = (int64_t)block * lanes; base < count; base += (int64_t)blocks * lanes) {
+        const int64_t i = base + l;
+        V v{};
+        if (i < count) v = sum_in_order(src + c0 * step + i, step, c1 - c0);
+        if (slices > 1) {
+            red[threadIdx.x] = v;
+            __syncthreads();
+            if (sl == 0)
+                for (int k = 1; k < slices; ++k) v += red[k * lanes + l];
+            __syncthreads();
+        }
+        if (sl == 0 && i < count) store(i, v);
+    }
+}
+// dW and db of the groups of several chunks = their partial sums, added in a fixed order.  blockIdx.y: which of those groups; the last blockIdx.x: db
 __global__ __launch_bounds__(256) void grouped_join_kernel(const GgP p) {
+    __shared__ f32x4 red[256];
     Tile t{};
     Groups<true> groups;
     if (!groups.several(p, p.chunk, threadIdx.x & 63, blockIdx.y, t)) return;
-    const int g = t.group, n = t.tiles;
+    const int g = t.group, n = t.tiles, blocks = gridDim.x - 1;
     const int64_t size = (int64_t)p.N * p.K;
     const float* const part = p.part + t.slot * size;
-    if (p.vec && (size & 3) == 0) {                                            // rows of whole 16-byte stores: so is the whole of dW_g
-        for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 1024) {
-            const f32x4 v = sum_in_order(reinterpret_cast<const f32x4*>(part + i), size / 4, n);
-            if (p.out16) *reinterpret_cast<uint2*>(p.out + (g * size + i) * 2) = make_uint2(bf_bits(v[0]) | (bf_bits(v[1]) << 16), bf_bits(v[2]) | (bf_bits(v[3]) << 16));
-            else *reinterpret_cast<f32x4*>(p.out + (g * size + i) * 4) = v;
-        }
-    } else {
-        for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-            const float v = sum_in_order(part + i, size, n);
-            if (p.out16) reinterpret_cast<bf16_t*>(p.out)[g * size + i] = (bf16_t)bf_bits(v);
-            else reinterpret_cast<float*>(p.out)[g * size + i] = v;
-        }
-    }
-    if (p.db != nullptr)
-        for (int c = blockIdx.x * 256 + threadIdx.x; c < p.N; c += gridDim.x * 256) {
-            const float v = sum_in_order(p.part_db + (int64_t)t.slot * p.N + c, p.N, n);
+    if ((int)blockIdx.x == blocks) {
+        if (p.db == nullptr) return;
+        join_sums(p.part_db + (int64_t)t.slot * p.N, p.N, p.N, n, 0, 1, reinterpret_cast<float*>(red), [&](int64_t c, float v) {
             if (p.bias16) ((bf16_t*)p.db)[(int64_t)g * p.N + c] = (bf16_t)bf_bits(v);
             else ((float*)p.db)[(int64_t)g * p.N + c] = v;
-        }
+        });
+    } else if (p.vec && (size & 3) == 0) {                                     // rows of whole 16-byte stores: so is the whole of dW_g
+        join_sums(reinterpret_cast<const f32x4*>(part), size / 4, size / 4, n, blockIdx.x, blocks, red, [&](int64_t i, const f32x4 v) {
+            if (p.out16) *reinterpret_cast<uint2*>(p.out + (g * size + 4 * i) * 2) = make_uint2(bf_bits(v[0]) | (bf_bits(v[1]) << 16), bf_bits(v[2]) | (bf_bits(v[3]) << 16));
+            else *reinterpret_cast<f32x4*>(p.out + (g * size + 4 * i) * 4) = v;
+        });
+    } else {
+        join_sums(part, size, size, n, blockIdx.x, blocks, reinterpret_cast<float*>(red), [&](int64_t i, float v) {
+            if (p.out16) reinterpret_cast<bf16_t*>(p.out)[g * size + i] = (bf16_t)bf_bits(v);
+            else reinterpret_cast<float*>(p.out)[g * size + i] = v;
+        });
+    }
 }
 
 // dst[r][0 .. 8 cpr) = src[r][0 .. cols), zeros behind: rows that begin on 16-byte boundaries (cpr chunks of 16 bytes each, one a thread)
@@ -876,9 +893,9 @@ extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x
     else if (h) go<bf16_t, WGRAD, 128, 128, 2, 2>(p, items, st);
     else go<float, WGRAD, 128, 128, 2, 2>(p, items, st);
     if (slots > 0) {
-        const int64_t nb = uem_cdiv((int64_t)N * K, 1024);
+        const int64_t chunks = uem_cdiv(T, p.chunk), nb = uem_cdiv((int64_t)N * K, chunks > 64 ? 64 : chunks > 16 ? 256 : 1024);
         const int64_t most = slots / 2 < G ? slots / 2 : G;                    // groups of several chunks
-        grouped_join_kernel<<<dim3((unsigned)(nb < 512 ? nb : 512), (unsigned)most), 256, 0, st>>>(p);
+        grouped_join_kernel<<<dim3((unsigned)(nb < 512 ? nb : 512) + 1, (unsigned)most), 256, 0, st>>>(p);
     }
     return uem_check_launch("grouped_wgrad");
 }
