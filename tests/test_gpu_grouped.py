@@ -97,6 +97,9 @@ SHAPES = [
     (4100, 40, 48, [4100], 0),
     (20000, 24, 16, [19000, 900], 3),                # and of many
     (20001, 23, 17, [20000], 1),
+    (50, 40, 1029, [20, 0, 29], 1),                  # few rows and a long reduction, forward and back
+    (70, 1031, 600, [33, 1, 0, 32], 0),
+    (3, 17, 2050, [1, 2], 0),
     (3500, 40, 136, [3] * 40 + [900] + [0] * 30 + [1100] + [5] * 20 + [256, 512, 300], 4),     # chunks and rests on both sides of lane 64
 ]
 

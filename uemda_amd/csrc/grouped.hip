@@ -614,40 +614,50 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
     }
 }
 
-// The forward of a few rows: the weights' bytes are all there is, and the latency of reaching them.  A tile is 32 rows x 32 columns, its
-// reduction shared out over sixteen waves that load their fragments straight into registers -- at 2048 channels a wave has all of its 8 KB
-// of W on the way at once -- and are joined through LDS in wave order.  Nine rows in six groups, 2048 -> 512: 13.5 -> 7.2 us.
-template <typename T>
+// The forward and the data gradient of a few rows: the weights' bytes are all there is, and the latency of reaching them.  A tile is 32 rows x
+// 32 columns, its reduction shared out over sixteen waves that load their fragments straight into registers -- at 2048 channels a wave has all
+// of its 8 KB of W on the way at once -- and are joined through LDS in wave order.  The data gradient's fragments of W are gathered element by
+// element, neighbouring lanes from neighbouring addresses.  Nine rows in six groups, 2048 -> 512: 13.5 -> 7.2 us.
+template <typename T, int FORM>
 __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
-    constexpr int ES = sizeof(T), PER = 16 / ES, NW = 16, LD = 36, DEEP = 8;   // LD: floats of a staged row, off the bank period
+    constexpr int ES = sizeof(T), PER = 16 / ES, NW = 16, LD = 36, DEEP = FORM == FWD ? 8 : 4;        // LD: floats of a staged row, off the bank period
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* const red = reinterpret_cast<float*>(smem);
     const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int width = FORM == FWD ? p.N : p.K, length = FORM == FWD ? p.K : p.N;
     Groups<false> groups;
     groups.init(p, 32, lane);
-    const int ct = (p.N + 31) / 32, item = xcd_item(groups.total * ct);
-    zero_rows<1024>(p, groups, p.N, groups.total * ct);
+    const int ct = (width + 31) / 32, item = xcd_item(groups.total * ct);
+    zero_rows<1024>(p, groups, width, groups.total * ct);
     if (item < 0) return;
     const Tile tl = groups.find(p, 32, lane, item / ct);
     const int c0 = (item % ct) * 32, r0 = tl.row0 + tl.tile * 32, rows = min(32, tl.rows - tl.tile * 32);
     // lanes of rows and columns past the end read the last one again; their results are not stored
     const char* const px = p.a + (int64_t)(r0 + min(fr, rows - 1)) * p.lda;
-    const char* const pw = p.b + ((int64_t)tl.group * p.N + min(c0 + fr, p.N - 1)) * p.ldb;
+    const int c = min(c0 + fr, width - 1);
+    const char* const pw = FORM == FWD ? p.b + ((int64_t)tl.group * p.N + c) * p.ldb : p.b + (int64_t)tl.group * p.N * p.ldb + c * ES;
     f32x16 acc;
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[r] = 0.f;
-    const int steps = (p.K + 2 * PER - 1) / (2 * PER);                         // a lane's 16 bytes are chunk 2 * step + fh
+    const int steps = (length + 2 * PER - 1) / (2 * PER);                      // a lane's 16 bytes are chunk 2 * step + fh
     for (int s0 = wave; s0 < steps; s0 += NW * DEEP) {
         Frag<T, false, 32> x[DEEP], w[DEEP];
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) {
-            const int chunk = 2 * (s0 + k * NW) + fh;
-            const bool on = chunk * PER < p.K;
+            const int at = (2 * (s0 + k * NW) + fh) * PER;
             const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-            const f32x4 vx = on ? *reinterpret_cast<const f32x4*>(px + chunk * 16) : zero, vw = on ? *reinterpret_cast<const f32x4*>(pw + chunk * 16) : zero;
+            const f32x4 vx = at < length ? *reinterpret_cast<const f32x4*>(px + at * ES) : zero;
             x[k].v = __builtin_bit_cast(decltype(x[k].v), vx);
-            w[k].v = __builtin_bit_cast(decltype(w[k].v), vw);
+            if (FORM == FWD) {
+                const f32x4 vw = at < length ? *reinterpret_cast<const f32x4*>(pw + at * ES) : zero;
+                w[k].v = __builtin_bit_cast(decltype(w[k].v), vw);
+            } else {
+                struct { T e[PER]; } vw;
+#pragma unroll
+                for (int e = 0; e < PER; ++e) vw.e[e] = at + e < length ? *reinterpret_cast<const T*>(pw + (int64_t)(at + e) * p.ldb) : (T)0;
+                w[k].v = __builtin_bit_cast(decltype(w[k].v), vw);
+            }
         }
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) mma(w[k], x[k], acc, T{});
@@ -657,7 +667,7 @@ __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
         *reinterpret_cast<f32x4*>(red + (wave * 32 + fr) * LD + 8 * h + 4 * fh) = f32x4{acc[4 * h], acc[4 * h + 1], acc[4 * h + 2], acc[4 * h + 3]};
     __syncthreads();
     const int m = threadIdx.x >> 5, n = threadIdx.x & 31;
-    if (m >= rows || c0 + n >= p.N) return;
+    if (m >= rows || c0 + n >= width) return;
     float v = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) v += red[(w * 32 + m) * LD + n];
@@ -792,19 +802,27 @@ int wgrad_chunk(int T, int G, int N, int K, int bm) {
 }
 int64_t wgrad_slots(int T, int chunk) { return T > chunk ? 2 * (int64_t)T / chunk : 0; }      // m > 1 chunks are of more than (m - 1) * chunk rows
 
-// 32 x 32 tiles of sixteen waves: while they are no more than the CUs and rows are long enough to share out.  Measured, us, tiles / these:
-// 6 groups 2048 -> 512 with 9, 256, 512 rows 13.5 / 7.2, 13.6 / 10.1, 14.1 / 17.8; 64 groups 1024 -> 1024 with 9, 64 rows (2048 tiles) 8.3 /
-// 10.5, 21.0 / 31.5; 8 groups 64 -> 64 3.8 / 4.5.
-bool few_rows(const GgP& p, int es) { return likely_tiles(p.T, p.G, 32) * uem_cdiv(p.N, 32) <= 256 && p.K * es >= 512; }
+// 32 x 32 tiles of sixteen waves: while they are few -- the larger tiles would leave most CUs idle, each block walking the whole reduction -- and
+// rows are long enough to share out.  Measured, us, the larger tiles / these, with these tiles' number in brackets:
+//   bf16 forward 2048 -> 512 14.8 / 7.4 (64), 14.8 / 10.2 (176), 15.0 / 18.6 (400); 1024 -> 1024 9.0 / 7.7 (384); 512 -> 512 6.1 / 5.1 (176);
+//     64 -> 1024 3.8 / 5.6 (160).  Data gradient, reduction 2048 14.6 / 7.8 (48), 15.0 / 16.8 (408); 1024 9.2 / 6.7 (192); 512 6.4 / 4.9 (80),
+//     6.9 / 8.3 (256); 256 5.4 / 7.6 (160).
+//   fp32 forward 2048 -> 512 72 / 25 (176), 74 / 66 (800), 76 / 126 (1552); 1024 -> 1024 38 / 14 (384), 40 / 35 (832); 512 -> 512 22 / 17 (400),
+//     22 / 27 (800); 256 -> 2048 11.5 / 7.2 (64), 11.6 / 13.0 (320); 64 -> 1024 5.2 / 8.5 (160).  Data gradient alike: 2048 72 / 21 (208), 1024 38 / 11 (54).
+bool few_rows(int64_t tiles, int length, bool is16, bool dgrad) {
+    if (is16) return length >= (dgrad ? 512 : 256) && tiles <= (dgrad && length < 1024 ? 128 : 256);
+    return length >= 128 && tiles <= (length >= 1024 ? 768 : length >= 512 ? 512 : 256);
+}
 template <typename T, int FORM>
 int launch_rows(const GgP& p, const char* what, hipStream_t st) {
-    if (FORM == FWD && few_rows(p, sizeof(T))) {
-        const int64_t items = (p.T / 32 + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(p.N, 32);
+    const int width = FORM == FWD ? p.N : p.K, length = FORM == FWD ? p.K : p.N;
+    if (few_rows(likely_tiles(p.T, p.G, 32) * uem_cdiv(width, 32), length, sizeof(T) == 2, FORM == DGRAD)) {
+        const int64_t items = (p.T / 32 + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(width, 32);
         constexpr int LDS = 16 * 32 * 36 * 4;
-        if (uem_allow_lds((const void*)grouped_few_kernel<T>, LDS)) grouped_few_kernel<T><<<(unsigned)(uem_cdiv(items, 8) * 8), 1024, LDS, st>>>(p);
+        if (uem_allow_lds((const void*)grouped_few_kernel<T, FORM>, LDS)) grouped_few_kernel<T, FORM><<<(unsigned)(uem_cdiv(items, 8) * 8), 1024, LDS, st>>>(p);
         return uem_check_launch(what);
     }
-    const int width = FORM == FWD ? p.N : p.K, t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
+    const int t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
     const int64_t items = (p.T / TILES[t].bm + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(width, TILES[t].bn);   // at most so many tiles: one of each group with rows is not full
     UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than the kernels count", what, (long long)items);
     if (sizeof(T) == 2 && t == 0) go<bf16_t, FORM, 256, 256, 2, 4>(p, items, st);
