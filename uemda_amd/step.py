@@ -251,6 +251,16 @@ def finish(aligner):
         aligner.check_superpixel_ids(wait=True)
 
 
+def retire_collectives():
+    """Waits until the RCCL process group's watchdog has let go of every collective issued so far (a host wait of at most some 100 ms once the
+    device is done with them).  Without such a group: nothing to wait for."""
+    import torch.distributed as dist
+    if not (dist.is_available() and dist.is_initialized()) or dist.get_backend() != "nccl":
+        return False
+    dist.group.WORLD._wait_for_pending_works()
+    return True
+
+
 class GraphedStep:
     """One whole training iteration captured in ONE hipGraph and replayed: ~1100 kernel launches per step become one graph launch
     (host time per step 0.2 ms instead of 16-30).  The device time is unchanged -- the step is device-bound at the benchmark batch --
@@ -324,7 +334,10 @@ class GraphedStep:
         # With a process group alive, its watchdog thread polls its work events (hipEventQuery) whenever it likes: under the default
         # "global" capture mode such a call from ANOTHER thread while this one captures is an error, raised in that thread -- the
         # process aborts, now and then (seen once in four runs of the captured data-parallel step).  "thread_local" checks this
-        # thread's calls only; what is recorded is the same (capture is per stream).
+        # thread's calls only; what is recorded is the same (capture is per stream).  And the eager steps' collectives, long done, stay on
+        # the watchdog's list until its next poll: their events were recorded on RCCL's stream, and once the capture reaches that stream a
+        # query of them is an error in either mode ("event last recorded in a capturing stream").  So the list is emptied first.
+        retire_collectives()
         mode = "thread_local" if (dp is not None or (torch.distributed.is_available() and torch.distributed.is_initialized())) else "global"
         if not graph_side:
             ops.SIDE_OFF += 1
