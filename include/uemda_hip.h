@@ -511,13 +511,15 @@ int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld
  * x, W, dy (and y, dx) are fp32, or bf16 with UEM_GROUPED_BF16; dW has their type, or fp32 with UEM_GROUPED_OUT_F32 (a bf16 product for an
  * fp32 master weight); bias / db are fp32, or bf16 with UEM_GROUPED_BIAS_BF16.  *_ld: row strides in ELEMENTS; rows of the operands must
  * begin on 16-byte boundaries and be followed by zeros up to the next one (whatever their stride holds beyond it) -- uem_grouped_pad copies
- * rows of any length to such a stride.  No group is read beyond its
+ * rows of any length to such a stride -- unless uem_grouped_any_rows (T rows in all; dgrad: of uem_grouped_dgrad, else of uem_grouped_fwd) says that calls of
+ * these sizes read rows that begin on any element, as those of few rows do.  No group is read beyond its
  * rows, sums run in a fixed order.  A size of the workspace goes with the flags of the call.                                      */
 #define UEM_GROUPED_BF16 1
 #define UEM_GROUPED_OUT_F32 2
 #define UEM_GROUPED_BIAS_BF16 4
 #define UEM_GROUPED_OFFSETS_64 8
 int uem_grouped_pad(const void* src, int64_t src_ld, void* dst, int dst_ld, int cols, int64_t rows, int flags, void* stream);
+int uem_grouped_any_rows(int T, int G, int K, int N, int flags, int dgrad);
 int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void* bias, void* y, const void* offsets, int T, int G, int K, int N,
                     int flags, void* stream);
 int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w_ld, void* dx, const void* offsets, int T, int G, int K, int N, int flags,

@@ -201,6 +201,28 @@ def test_strides_and_starts(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K,N", [(601, 523), (1031, 40), (44, 1543), (1030, 1030)])
+def test_few_rows_that_begin_on_any_element(K, N, dtype):
+    """rows and weights are read where they lie, forward and back: slices of wider buffers, whose rows start anywhere and end in what must not count"""
+    T, G = 12, 3
+    o = edges(T, [5, 0, 6], 1)
+    x, w, b, dy = data(T, G, K, N, dtype, K)
+    y0, g0 = check(x, w, b, dy, o)
+    for pad, start in ((3, 1), (1, 0), (8, 5)):
+        wide = torch.full((T, K + pad + start), float("nan"), device="cuda", dtype=dtype)
+        wide[:, start:start + K] = x
+        wdy = torch.full((T, N + pad + start), float("inf"), device="cuda", dtype=dtype)
+        wdy[:, start:start + N] = dy
+        ww = torch.full((G, N, K + pad + start), float("nan"), device="cuda", dtype=dtype)
+        ww[:, :, start:start + K] = w
+        y, g = check(wide[:, start:start + K], ww[:, :, start:start + K], b, wdy[:, start:start + N], o)
+        assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(g, g0))
+    from uemda_amd.grouped import grouped_linear
+    off, xl = torch.tensor(o, device="cuda"), x.clone().requires_grad_()      # the data gradient alone: dy is not copied either
+    assert torch.equal(torch.autograd.grad(grouped_linear(xl, w, off, b), xl, wdy[:, start:start + N])[0], g0[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_rows_of_no_group_and_of_other_groups_do_not_leak(dtype):
     from uemda_amd.grouped import grouped_linear
     T, K, N = 400, 72, 88

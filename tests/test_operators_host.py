@@ -102,6 +102,10 @@ def test_grouped_linear_refusals():
     lib = _lib.load()
     assert lib.uem_grouped_fwd(None, 8, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1
     assert lib.uem_grouped_fwd(16, 6, 16, 8, None, 16, 16, 4, 2, 6, 8, 0, None) == -1 and b"16-byte" in lib.uem_last_error()
+    assert lib.uem_grouped_any_rows(4, 2, 6, 8, 0, 0) == 0 and lib.uem_grouped_any_rows(4, 2, 600, 8, 0, 0) == 1          # few rows, long ones
+    assert lib.uem_grouped_any_rows(4, 2, 600, 8, 0, 1) == 0 and lib.uem_grouped_any_rows(4, 2, 8, 600, 0, 1) == 1
+    assert lib.uem_grouped_any_rows(10 ** 6, 2, 600, 8, 0, 0) == 0
+    assert lib.uem_grouped_fwd(18, 600, 16, 600, None, 16, 16, 4, 2, 600, 8, 0, None) == -1 and b"element" in lib.uem_last_error()
     assert lib.uem_grouped_fwd(24, 8, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1
     assert lib.uem_grouped_fwd(16, 4, 16, 8, None, 16, 16, 4, 2, 8, 8, 0, None) == -1 and b"shorter" in lib.uem_last_error()
     assert lib.uem_grouped_fwd(16, 8, 16, 8, None, 16, 16, 1 << 30, 2, 8, 8, 0, None) == -1

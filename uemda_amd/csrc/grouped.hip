@@ -617,10 +617,17 @@ __global__ __launch_bounds__(64 * WGM * WGN, 2) void grouped_kernel(const GgP p)
 // The forward and the data gradient of a few rows: the weights' bytes are all there is, and the latency of reaching them.  A tile is 32 rows x
 // 32 columns, its reduction shared out over sixteen waves that load their fragments straight into registers -- at 2048 channels a wave has all
 // of its 8 KB of W on the way at once -- and are joined through LDS in wave order.  The data gradient's fragments of W are gathered element by
-// element, neighbouring lanes from neighbouring addresses.  Nine rows in six groups, 2048 -> 512: 13.5 -> 7.2 us.
+// element, neighbouring lanes from neighbouring addresses.  Rows may begin on any element: a copy of W to padded rows would cost its bytes twice
+// over (one row, 27 groups, 1358 -> 1414 bf16, a training step 147 us, so 85).  Nine rows in six groups, 2048 -> 512: 13.5 -> 7.2 us.
 template <typename T, int FORM>
 __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
     constexpr int ES = sizeof(T), PER = 16 / ES, NW = 16, LD = 36, DEEP = FORM == FWD ? 8 : 4;        // LD: floats of a staged row, off the bank period
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    struct __attribute__((packed, aligned(ES))) Chunk { unsigned w[4]; };                             // 16 bytes of a row, on any element boundary
+    auto chunk = [](const char* q) {
+        const Chunk c = *reinterpret_cast<const Chunk*>(q);
+        return u32x4{c.w[0], c.w[1], c.w[2], c.w[3]};
+    };
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* const red = reinterpret_cast<float*>(smem);
     const int lane = threadIdx.x & 63, fr = lane & 31, fh = lane >> 5;
@@ -645,22 +652,32 @@ __global__ __launch_bounds__(1024) void grouped_few_kernel(const GgP p) {
         Frag<T, false, 32> x[DEEP], w[DEEP];
 #pragma unroll
         for (int k = 0; k < DEEP; ++k) {
-            const int at = (2 * (s0 + k * NW) + fh) * PER;
-            const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-            const f32x4 vx = at < length ? *reinterpret_cast<const f32x4*>(px + at * ES) : zero;
-            x[k].v = __builtin_bit_cast(decltype(x[k].v), vx);
-            if (FORM == FWD) {
-                const f32x4 vw = at < length ? *reinterpret_cast<const f32x4*>(pw + at * ES) : zero;
-                w[k].v = __builtin_bit_cast(decltype(w[k].v), vw);
-            } else {
-                struct { T e[PER]; } vw;
+            // the last chunk that lies inside the row stands in for those past its end, without what the chunk in front of it holds already
+            if (s0 + k * NW >= steps) continue;
+            const int from = min((2 * (s0 + k * NW) + fh) * PER, length - PER);
+            x[k].v = __builtin_bit_cast(decltype(x[k].v), chunk(px + from * ES));
+            if (FORM == FWD) w[k].v = __builtin_bit_cast(decltype(w[k].v), chunk(pw + from * ES));
+            else {
+                struct { T e[PER]; } c;
 #pragma unroll
-                for (int e = 0; e < PER; ++e) vw.e[e] = at + e < length ? *reinterpret_cast<const T*>(pw + (int64_t)(at + e) * p.ldb) : (T)0;
-                w[k].v = __builtin_bit_cast(decltype(w[k].v), vw);
+                for (int e = 0; e < PER; ++e) c.e[e] = *reinterpret_cast<const T*>(pw + (int64_t)(from + e) * p.ldb);
+                w[k].v = __builtin_bit_cast(decltype(w[k].v), c);
             }
         }
+        __builtin_amdgcn_sched_barrier(0);                                     // all of them on their way before the first is waited for
 #pragma unroll
-        for (int k = 0; k < DEEP; ++k) mma(w[k], x[k], acc, T{});
+        for (int k = 0; k < DEEP; ++k) {
+            if (s0 + k * NW != steps - 1) continue;                            // (uniform) the chunks of both halves exist, or neither
+            const int at = (2 * (s0 + k * NW) + fh) * PER, skip = at - min(at, length - PER);
+            u32x4 keep;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) keep[j] = ES == 4 ? (j >= skip ? ~0u : 0u) : (2 * j >= skip ? 0xffffu : 0u) | (2 * j + 1 >= skip ? 0xffff0000u : 0u);
+            x[k].v = __builtin_bit_cast(decltype(x[k].v), __builtin_bit_cast(u32x4, x[k].v) & keep);
+            w[k].v = __builtin_bit_cast(decltype(w[k].v), __builtin_bit_cast(u32x4, w[k].v) & keep);
+        }
+#pragma unroll
+        for (int k = 0; k < DEEP; ++k)
+            if (s0 + k * NW < steps) mma(w[k], x[k], acc, T{});
     }
 #pragma unroll
     for (int h = 0; h < 4; ++h)                                                // rows of the result: columns 8 h + 4 fh + 0 .. 3 of feature row fr
@@ -813,10 +830,14 @@ bool few_rows(int64_t tiles, int length, bool is16, bool dgrad) {
     if (is16) return length >= (dgrad ? 512 : 256) && tiles <= (dgrad && length < 1024 ? 128 : 256);
     return length >= 128 && tiles <= (length >= 1024 ? 768 : length >= 512 ? 512 : 256);
 }
+template <int FORM> bool takes_few(int T, int G, int K, int N, bool is16) {
+    const int width = FORM == FWD ? N : K;
+    return FORM != WGRAD && few_rows(likely_tiles(T, G, 32) * uem_cdiv(width, 32), FORM == FWD ? K : N, is16, FORM == DGRAD);
+}
 template <typename T, int FORM>
 int launch_rows(const GgP& p, const char* what, hipStream_t st) {
-    const int width = FORM == FWD ? p.N : p.K, length = FORM == FWD ? p.K : p.N;
-    if (few_rows(likely_tiles(p.T, p.G, 32) * uem_cdiv(width, 32), length, sizeof(T) == 2, FORM == DGRAD)) {
+    const int width = FORM == FWD ? p.N : p.K;
+    if (takes_few<FORM>(p.T, p.G, p.K, p.N, sizeof(T) == 2)) {
         const int64_t items = (p.T / 32 + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(width, 32);
         constexpr int LDS = 16 * 32 * 36 * 4;
         if (uem_allow_lds((const void*)grouped_few_kernel<T, FORM>, LDS)) grouped_few_kernel<T, FORM><<<(unsigned)(uem_cdiv(items, 8) * 8), 1024, LDS, st>>>(p);
@@ -831,13 +852,16 @@ int launch_rows(const GgP& p, const char* what, hipStream_t st) {
     return uem_check_launch(what);
 }
 
+template <int FORM>
 int check(const void* a, const void* b, const void* out, const void* offsets, int T, int G, int K, int N, int lda, int ldb, int flags, const char* what) {
     const int es = (flags & UEM_GROUPED_BF16) ? 2 : 4;
     UEM_REQUIRE(a && b && out && offsets, "%s: null pointer", what);
     UEM_REQUIRE(T > 0 && G > 0 && K > 0 && N > 0 && T < (1 << 30) && G < (1 << 16) && K <= (1 << 20) && N <= (1 << 20),
                 "%s: rows < 2^30, groups < 65536, K and N <= 2^20 (got %d, %d, %d, %d)", what, T, G, K, N);
-    UEM_REQUIRE((((uintptr_t)a | (uintptr_t)b) & 15) == 0 && (int64_t)lda * es % 16 == 0 && (int64_t)ldb * es % 16 == 0,
-                "%s: operand rows must begin on 16-byte boundaries (uem_grouped_pad)", what);
+    const uintptr_t at = (uintptr_t)a | (uintptr_t)b;
+    if (takes_few<FORM>(T, G, K, N, es == 2)) UEM_REQUIRE(at % es == 0, "%s: operands must begin on element boundaries", what);
+    else UEM_REQUIRE((at & 15) == 0 && (int64_t)lda * es % 16 == 0 && (int64_t)ldb * es % 16 == 0,
+                     "%s: operand rows must begin on 16-byte boundaries (uem_grouped_pad)", what);
     UEM_REQUIRE((int64_t)lda * es <= (1 << 23) && (int64_t)ldb * es <= (1 << 23), "%s: row strides of at most 8 MB", what);
     UEM_REQUIRE((flags & ~(UEM_GROUPED_BF16 | UEM_GROUPED_OUT_F32 | UEM_GROUPED_BIAS_BF16 | UEM_GROUPED_OFFSETS_64)) == 0, "%s: unknown flags %d", what, flags);
     return UEM_OK;
@@ -868,9 +892,13 @@ extern "C" int uem_grouped_pad(const void* src, int64_t src_ld, void* dst, int d
     else grouped_pad_kernel<float><<<grid, 256, 0, st>>>((const float*)src, src_ld, (float*)dst, dst_ld / per, cols, chunks);
     return uem_check_launch("grouped_pad");
 }
+extern "C" int uem_grouped_any_rows(int T, int G, int K, int N, int flags, int dgrad) {
+    const bool is16 = (flags & UEM_GROUPED_BF16) != 0;
+    return dgrad ? takes_few<DGRAD>(T, G, K, N, is16) : takes_few<FWD>(T, G, K, N, is16);
+}
 extern "C" int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void* bias, void* y, const void* offsets, int T, int G, int K,
                                int N, int flags, void* stream) {
-    const int rc = check(x, w, y, offsets, T, G, K, N, x_ld, w_ld, flags, "grouped_fwd");
+    const int rc = check<FWD>(x, w, y, offsets, T, G, K, N, x_ld, w_ld, flags, "grouped_fwd");
     if (rc != UEM_OK) return rc;
     UEM_REQUIRE(x_ld >= K && w_ld >= K, "grouped_fwd: row strides shorter than the rows");
     GgP p = params(x, x_ld, w, w_ld, y, N, offsets, T, G, K, N, flags);
@@ -880,7 +908,7 @@ extern "C" int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld,
 }
 extern "C" int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w_ld, void* dx, const void* offsets, int T, int G, int K, int N, int flags,
                                  void* stream) {
-    const int rc = check(dy, w, dx, offsets, T, G, K, N, dy_ld, w_ld, flags, "grouped_dgrad");
+    const int rc = check<DGRAD>(dy, w, dx, offsets, T, G, K, N, dy_ld, w_ld, flags, "grouped_dgrad");
     if (rc != UEM_OK) return rc;
     UEM_REQUIRE(dy_ld >= N && w_ld >= K, "grouped_dgrad: row strides shorter than the rows");
     const GgP p = params(dy, dy_ld, w, w_ld, dx, K, offsets, T, G, K, N, flags);
@@ -893,7 +921,7 @@ extern "C" int64_t uem_grouped_wgrad_workspace_floats(int T, int G, int K, int N
 }
 extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x_ld, void* dw, void* db, float* workspace, const void* offsets, int T,
                                  int G, int K, int N, int flags, void* stream) {
-    const int rc = check(dy, x, dw, offsets, T, G, K, N, dy_ld, x_ld, flags, "grouped_wgrad");
+    const int rc = check<WGRAD>(dy, x, dw, offsets, T, G, K, N, dy_ld, x_ld, flags, "grouped_wgrad");
     if (rc != UEM_OK) return rc;
     UEM_REQUIRE(dy_ld >= N && x_ld >= K, "grouped_wgrad: row strides shorter than the rows");
     hipStream_t st = (hipStream_t)stream;

@@ -47,7 +47,7 @@ template <typename... A> [[noreturn]] void refuse(const A&... a) {
 // ---- the C ABI --------------------------------------------------------------------------------------------------------------------------
 #define UEM_HOST_FUNCTIONS(F) \
     F(uem_last_error) F(uem_layernorm_workspace_floats) F(uem_layernorm_fwd) F(uem_layernorm_bwd) F(uem_multi_norm_workspace_doubles) \
-    F(uem_multi_norm) F(uem_multi_clip) F(uem_grouped_pad) F(uem_grouped_fwd) F(uem_grouped_dgrad) F(uem_grouped_wgrad_workspace_floats) \
+    F(uem_multi_norm) F(uem_multi_clip) F(uem_grouped_pad) F(uem_grouped_any_rows) F(uem_grouped_fwd) F(uem_grouped_dgrad) F(uem_grouped_wgrad_workspace_floats) \
     F(uem_grouped_wgrad) F(uem_cast_f32_bf16)
 #define UEM_DECLARE(name) decltype(&::name) name##_ = nullptr;
 UEM_HOST_FUNCTIONS(UEM_DECLARE)
@@ -174,22 +174,21 @@ Tensor layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
 
 // ---- grouped products -------------------------------------------------------------------------------------------------------------------
 constexpr int64_t MOST_LD = 1 << 21;              // elements between rows that the kernels address
-// 2-d t as rows that begin on 16-byte boundaries and end in zeros up to the next: t itself, or a copy
-Tensor operand(Tensor t, int& ld) {
+// 2-d t as rows that begin on 16-byte boundaries and end in zeros up to the next -- `any`: on any element -- t itself, or a copy
+Tensor operand(Tensor t, int& ld, bool any = false) {
     const int64_t rows = t.size(0), cols = t.size(1), per = 16 / t.element_size();
     if ((cols > 1 && t.stride(1) != 1) || (rows > 1 && !(cols <= t.stride(0) && t.stride(0) <= MOST_LD))) t = t.contiguous();
     const int64_t have = rows > 1 ? t.stride(0) : cols;
-    if (cols % per == 0 && have % per == 0 && ((uintptr_t)t.const_data_ptr() & 15) == 0) { ld = (int)have; return t; }
+    if (any || (cols % per == 0 && have % per == 0 && ((uintptr_t)t.const_data_ptr() & 15) == 0)) { ld = (int)have; return t; }
     ld = (int)((cols + per - 1) / per * per);
     const Tensor out = at::empty({rows, ld}, t.options());
     CALL(uem_grouped_pad, ptr(t), have, mptr(out), ld, (int)cols, rows, is16(t) ? UEM_GROUPED_BF16 : 0, stream_of(t));
     return out;
 }
-int row_stride(const Tensor& o) { return (int)(o.size(0) > 1 ? o.stride(0) : o.size(1)); }      // of what operand() returned
 int grouped_flags(const Tensor& x, const Tensor& offsets) {
     return (is16(x) ? UEM_GROUPED_BF16 : 0) | (offsets.scalar_type() == at::kLong ? UEM_GROUPED_OFFSETS_64 : 0);
 }
-struct Grouped { Tensor y, x, w; };               // y, and the operands as the kernels read them
+struct Grouped { Tensor y, x, w; };               // y, and the operands as the forward's kernel reads them
 Grouped grouped_forward(const Tensor& x, const Tensor& weight, const Tensor& offsets, const Tensor& bias) {
     const c10::DeviceGuard guard(x.device());
     const int64_t T = x.size(0), K = x.size(1), G = weight.size(0), N = weight.size(1);
@@ -203,10 +202,12 @@ Grouped grouped_forward(const Tensor& x, const Tensor& weight, const Tensor& off
         w = w16;
     }
     int x_ld, w_ld;
-    r.x = operand(x, x_ld);
-    r.w = operand(w, w_ld);
+    const int flags = grouped_flags(x, offsets);
+    const bool any = uem_grouped_any_rows_((int)T, (int)G, (int)K, (int)N, flags, 0) != 0;
+    r.x = operand(x, x_ld, any);
+    r.w = operand(w, w_ld, any);
     CALL(uem_grouped_fwd, ptr(r.x), x_ld, ptr(r.w), w_ld, ptr(bias), mptr(r.y), ptr(offsets), (int)T, (int)G, (int)K, (int)N,
-         grouped_flags(x, offsets) | (is16(bias) ? UEM_GROUPED_BIAS_BF16 : 0), stream_of(x));
+         flags | (is16(bias) ? UEM_GROUPED_BIAS_BF16 : 0), stream_of(x));
     return r;
 }
 struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
@@ -237,15 +238,20 @@ struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
             if (need_w) dw.zero_();
             if (need_b) db.zero_();
         } else {
-            int dy_ld;
-            const Tensor dy = operand(grads[0], dy_ld);
             const int flags = grouped_flags(x, offsets);
-            if (need_x) CALL(uem_grouped_dgrad, ptr(dy), dy_ld, ptr(w), row_stride(w), mptr(dx), ptr(offsets), T, G, K, N, flags, stream_of(x));
+            const bool any = uem_grouped_any_rows_(T, G, K, N, flags, 1) != 0;
+            int dy_ld, w_ld, x_ld;
+            const Tensor dy = operand(grads[0], dy_ld, any && !need_w && !need_b);
+            if (need_x) {
+                const Tensor wr = operand(w, w_ld, any);
+                CALL(uem_grouped_dgrad, ptr(dy), dy_ld, ptr(wr), w_ld, mptr(dx), ptr(offsets), T, G, K, N, flags, stream_of(x));
+            }
             if (need_w || need_b) {
                 const int64_t n = uem_grouped_wgrad_workspace_floats_(T, G, K, N, flags);
                 Tensor ws;
                 if (n > 0) ws = at::empty({n}, x.options().dtype(at::kFloat));
-                CALL(uem_grouped_wgrad, ptr(dy), dy_ld, ptr(x), row_stride(x), mptr(dw), mptr(db), (float*)mptr(ws), ptr(offsets), T, G, K, N,
+                const Tensor xr = operand(x, x_ld);
+                CALL(uem_grouped_wgrad, ptr(dy), dy_ld, ptr(xr), x_ld, mptr(dw), mptr(db), (float*)mptr(ws), ptr(offsets), T, G, K, N,
                      flags | (w16 ? 0 : UEM_GROUPED_OUT_F32) | (b16 ? UEM_GROUPED_BIAS_BF16 : 0), stream_of(x));
             }
         }
