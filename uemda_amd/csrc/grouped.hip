@@ -12,8 +12,8 @@
 // 16-byte chunks on the source address so that a read covers all banks.  Buffer descriptors that end with the group's last row (and
 // offsets beyond them for columns past the end) supply the zeros of every ragged edge: no row of another group is ever read.
 // Products are exact in the fp32 accumulators (bf16) or fp32 MFMA (fp32); bf16 results are rounded once.
-// Measured, bf16, 65536 x 2048 -> 2048 in 32 ragged groups, us: forward 505 - 545, data gradient 495 - 516, weight gradient with db 483 - 510
-// (550 GFLOP each: 1.01 - 1.14 PFLOP/s; in groups of 2048 rows 470 = 1.17, a dense library product of the size 467): the clock falls to 1.7 GHz under the products, what
+// Measured, bf16, 65536 x 2048 -> 2048 in 32 ragged groups, us: forward 485 - 520, data gradient 480 - 515, weight gradient with db 485 - 510
+// (550 GFLOP each: 1.06 - 1.15 PFLOP/s; in groups of 2048 rows 470 = 1.17, a dense library product of the size 467): the clock falls to 1.7 GHz under the products, what
 // is left is a tile's start and end.  fp32, 65536 x 2048 -> 2048 in 8 groups: 3.9 ms = 142 TFLOP/s of the 151 a dense product reaches.
 //
 // Nothing is read on the host: a block finds its tiles by prefix sums over the offsets, 64 groups to a wave, kept in registers.  Offsets are clamped to [0, T] and to the largest one in front of them, so that any
