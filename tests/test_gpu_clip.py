@@ -219,3 +219,43 @@ def test_a_model_arena_together_with_other_modules():
     assert abs(float(n) / both - 1) < 1e-6
     for b, p in zip(before, list(model.parameters()) + list(head.parameters())):
         torch.testing.assert_close(p.grad, b * (32.0 / both), rtol=1e-6, atol=0)
+
+
+def test_some_of_a_models_parameters_are_clipped_alone():
+    """a single parameter, a list of some, the largest magnitude of all: only what is listed is measured and scaled; the list of all that is
+    trained gives what the model's arena gives"""
+    from uemda_amd.models.Encoder import Deeplabv2
+    from uemda_amd.optim import clip_grad_norm_, grad_norm
+    torch.manual_seed(0)
+    model = Deeplabv2(dict(backbone=dict(resnet_type="resnet50", output_stride=16, pretrained=False), multi_layer=True, cascade=False, use_ppm=False,
+                           ppm=dict(num_classes=6, use_aux=False, fc_dim=2048), inchannels=2048, num_classes=6, is_ins_norm=True)).cuda()
+    model.zero_grad()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    params = list(model.parameters())
+
+    def fill():
+        for p in params:
+            p.grad.copy_(torch.randn(p.shape, generator=g, device="cuda"))
+    for listed in (params[7], params[:1], params[3:90], params[1:]):
+        fill()
+        names = {id(p) for p in ([listed] if isinstance(listed, torch.Tensor) else listed)}
+        before = [p.grad.clone() for p in params]
+        want = exact_norm([b for b, p in zip(before, params) if id(p) in names], 2)
+        n = clip_grad_norm_(listed, 0.5)
+        assert abs(float(n) - want) <= 2.0 ** -23 * want
+        for b, p in zip(before, params):                       # the coefficient and the product: 5 roundings of half a step
+            ref = b.double() * (0.5 / (want + 1e-6)) if id(p) in names else b.double()
+            assert ((p.grad.double() - ref).abs() <= ref.abs() * (5 * 2.0 ** -24 if id(p) in names else 0)).all()
+    fill()
+    before = [p.grad.clone() for p in params]
+    want = exact_norm(before, 0)
+    assert float(clip_grad_norm_(params, 0.5, INF)) == want
+    for b, p in zip(before, params):
+        ref = b.double() * (0.5 / (want + 1e-6))
+        assert ((p.grad.double() - ref).abs() <= ref.abs() * (5 * 2.0 ** -24)).all()
+    fill()
+    before, alone = [p.grad.clone() for p in params], grad_norm(model)[0].clone()
+    assert torch.equal(clip_grad_norm_(filter(lambda p: p.requires_grad, params), 32.0), alone)
+    coef = torch.clamp(32.0 / (alone + 1e-6), max=1.0)
+    for b, p in zip(before, params):
+        assert torch.equal(p.grad, b * coef)

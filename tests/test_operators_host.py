@@ -122,3 +122,33 @@ def test_the_host_extension_needs_its_binding():
     import sys
     code = "import torch\nfrom uemda_amd import _host\ntry:\n    _host.layer_norm(torch.zeros(2, 8), None, None, 1e-5)\nexcept RuntimeError as e:\n    assert 'bound' in str(e)\nelse:\n    raise SystemExit(1)"
     assert subprocess.run([sys.executable, "-c", code]).returncode == 0
+
+
+def test_only_a_whole_model_takes_its_arena(monkeypatch):
+    """a model's arena is clipped where the list is all that the model trains; some of its parameters are a list like any other"""
+    from uemda_amd import optim
+
+    class Model(torch.nn.Linear):
+        def flat_parameters(self):
+            raise LookupError("arena")
+    lists = []
+    monkeypatch.setattr(_lib, "host", lambda: type("host", (), {"multi_norm": staticmethod(lambda ps, *a: lists.append(ps) or torch.tensor(1.0))}))
+    m, other = Model(3, 2), torch.ones(2, requires_grad=True)
+    for p in m.parameters():
+        p._uem_owner, p.grad = m, torch.ones_like(p)
+    w, b = m.parameters()
+    for some in (w, [w], [b], [w, b, other], iter([b])):
+        assert float(optim.clip_grad_norm_(some, 1.0)) == 1.0
+    assert [len(ps) for ps in lists] == [1, 1, 1, 3, 1] and lists[0][0] is w and lists[4][0] is b
+    assert float(optim.clip_grad_norm_([w, b], 1.0, float("inf"))) == 1.0 and len(lists) == 6
+    b.requires_grad_(False)
+    optim.clip_grad_norm_([w], 1.0)                            # b is frozen, but what it holds is no gradient of the list
+    assert len(lists) == 7
+    b.grad = None
+    for whole in ([w], [w, b], m.parameters(), filter(lambda p: p.requires_grad, m.parameters())):
+        with pytest.raises(LookupError, match="arena"):
+            optim.clip_grad_norm_(whole, 1.0)
+    for bad in (-1.0, float("nan")):
+        with pytest.raises(UemError, match="negative"):
+            optim.clip_grad_norm_([w, b], bad)
+    assert len(lists) == 7

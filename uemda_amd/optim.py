@@ -7,9 +7,13 @@ from .ops import UemError, call, ptr, stream
 
 
 def _arena_of(params):
-    """the model whose flat arenas hold all of `params`, or None"""
+    """the model whose flat gradient arena IS the gradients of `params`: all of them are its parameters, and none that it trains or that
+    has a gradient is missing (frozen ones may be, as in `filter(lambda p: p.requires_grad, model.parameters())`).  Else None"""
     owner = getattr(params[0], "_uem_owner", None) if params else None
-    return owner if owner is not None and all(getattr(p, "_uem_owner", None) is owner for p in params) else None
+    if owner is None or any(getattr(p, "_uem_owner", None) is not owner for p in params):
+        return None
+    listed = {id(p) for p in params}
+    return owner if all(id(p) in listed or not (p.requires_grad or p.grad is not None) for p in owner.parameters()) else None
 
 
 def grad_norm(model):
@@ -41,25 +45,22 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2):
     """Drop-in for torch.nn.utils.clip_grad_norm_: scales the gradients of `parameters` (a tensor or an iterable) in place by
     min(max_norm / (norm + 1e-6), 1) and returns their total norm, a device scalar; norm_type is 2 or inf.
 
-    Parameters of ONE uemda_amd model: the model's whole flat gradient arena is clipped (norm_type 2).  Any other list -- modules outside a
-    model arena, or a model together with other modules, fp32 and bf16 mixed -- is clipped tensor by tensor in two passes over the list;
-    parameters without a gradient are skipped, gradients that share memory are refused."""
+    ALL trained parameters of one uemda_amd model: its flat gradient arena is clipped in one pass.  Any other list -- some of a model's
+    parameters, modules outside a model arena, a model together with other modules, fp32 and bf16 mixed -- is clipped tensor by tensor in
+    two passes over the list, and nothing beside it; parameters without a gradient are skipped, gradients that share memory are refused."""
     what = "clip_grad_norm_"
     params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
-    model = _arena_of(params)
+    kind, max_norm = _norm_kind(norm_type, what), float(max_norm)
+    if not max_norm >= 0.0:
+        raise UemError(f"{what}: max_norm must not be negative, got {max_norm}")
+    model = _arena_of(params) if kind == 2 else None
+    ops.grad_join()                # weight gradients still on the side / second stream (a backward that raised never ran its join callback)
     if model is None:
-        kind, max_norm = _norm_kind(norm_type, what), float(max_norm)
-        if not max_norm >= 0.0:
-            raise UemError(f"{what}: max_norm must not be negative, got {max_norm}")
-        ops.grad_join()            # gradients of arena parameters among them may still be on the side / second stream
         norm = _lib.host().multi_norm(params, what, kind, True, max_norm)
         return torch.zeros((), device=params[0].device if params else "cpu") if norm is None else norm
-    if norm_type != 2:
-        raise UemError("clip_grad_norm_: only the L2 norm is implemented for a model's flat arena")
     arena, garena, n = model.flat_parameters()
-    ops.grad_join()                # weight gradients still on the side / second stream (a backward that raised never ran its join callback)
     norm = grad_norm(model)
-    coef = torch.clamp(float(max_norm) / (norm + 1e-6), max=1.0)      # one scalar
+    coef = torch.clamp(max_norm / (norm + 1e-6), max=1.0)      # one scalar
     call("uem_scale_by_scalar", ptr(garena), None, n, ptr(coef), stream())
     return norm[0]
 
