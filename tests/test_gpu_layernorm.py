@@ -304,3 +304,19 @@ def test_results_repeat_and_a_captured_step_replays():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(held, want)), k
+
+
+def test_a_gradient_with_a_tangent_is_refused():
+    """forward mode over a backward pass: the node's kernels would drop the tangent of dy"""
+    import torch.autograd.forward_ad as fa
+
+    from uemda_amd import UemError
+    from uemda_amd.grouped import grouped_linear
+    from uemda_amd.norm import layer_norm
+    x = torch.randn(6, 8, device="cuda", requires_grad=True)
+    w, off = torch.randn(2, 4, 8, device="cuda"), torch.tensor([0, 3, 6], device="cuda")
+    for y in (layer_norm(x), grouped_linear(x, w, off)):
+        with fa.dual_level():
+            with pytest.raises(UemError, match="forward-mode"):
+                torch.autograd.grad(y, x, fa.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
+        assert torch.autograd.grad(y, x, torch.ones_like(y))[0].isfinite().all()

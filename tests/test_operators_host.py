@@ -152,3 +152,29 @@ def test_only_a_whole_model_takes_its_arena(monkeypatch):
         with pytest.raises(UemError, match="negative"):
             optim.clip_grad_norm_([w, b], bad)
     assert len(lists) == 7
+
+
+def test_forward_mode_and_traces_are_refused():
+    """a call without requires_grad does not reach the autograd node: nothing but the operator itself can see a tangent that it would drop"""
+    import torch.autograd.forward_ad as fa
+
+    from uemda_amd.grouped import grouped_linear
+    from uemda_amd.norm import layer_norm
+    from uemda_amd.optim import clip_grad_norm_, get_total_norm
+    x, w, b = torch.ones(6, 8), torch.ones(8), torch.zeros(8)
+    gw, gb, off = torch.ones(2, 4, 8), torch.zeros(2, 4), torch.tensor([0, 3, 6])
+    p = torch.ones(3, requires_grad=True)
+    with fa.dual_level():
+        dual = lambda t: fa.make_dual(t, torch.ones_like(t))
+        p.grad = dual(torch.ones(3))
+        calls = [lambda: layer_norm(dual(x), w, b), lambda: layer_norm(x, dual(w), b), lambda: layer_norm(x, w, dual(b)), lambda: layer_norm(dual(x)),
+                 lambda: grouped_linear(dual(x), gw, off, gb), lambda: grouped_linear(x, dual(gw), off), lambda: grouped_linear(x, gw, off, dual(gb)),
+                 lambda: get_total_norm([dual(w)]), lambda: clip_grad_norm_([p], 1.0)]
+        for k, call in enumerate(calls):
+            with pytest.raises(UemError, match="forward-mode"):
+                call()
+                pytest.fail(str(k))
+    p.grad = None
+    for fn, args in ((layer_norm, (x,)), (lambda a: layer_norm(a, w, b), (x,)), (grouped_linear, (x, gw, off)), (lambda a: get_total_norm([a]), (x,))):
+        with pytest.raises(UemError, match="traced"):
+            torch.jit.trace(fn, args)

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <cmath>
@@ -77,6 +78,14 @@ void no_second_derivative(const char* what) {
     if (at::GradMode::is_enabled()) refuse(what, ": a gradient of the gradient is not offered (create_graph=True)");
 }
 
+// Forward-mode derivatives and traces would pass the kernels by as silently: a dual tensor's tangent counts as zero in the result, and a trace
+// records the allocation of the output and no launch.  (A call without requires_grad never reaches the autograd node, which would refuse.)
+void no_transforms(const char* what, std::initializer_list<const Tensor*> list) {
+    if (torch::jit::tracer::isTracing()) refuse(what, ": its kernels cannot be traced (torch.jit.trace)");
+    for (const Tensor* t : list)
+        if (t->defined() && t->_fw_grad(0).defined()) refuse(what, ": a forward-mode derivative is not offered (a tensor of torch.autograd.forward_ad)");
+}
+
 // A graph of the same leaves that lives outside a capture holds the nodes that add up their gradients, on the stream they were made on; a
 // backward pass captured on another stream would join that stream to the capture, inside the engine, which ends the process.
 void no_outside_graph(const char* what, std::initializer_list<const Tensor*> list) {
@@ -127,6 +136,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         no_second_derivative("layer_norm");
+        no_transforms("layer_norm", {&grads[0]});
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
         const c10::DeviceGuard guard(x.device());
@@ -154,6 +164,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 };
 Tensor layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps) {
     if (!is_real(x)) refuse("layer_norm: x must be a float32 or bfloat16 tensor, got ", x.scalar_type());
+    no_transforms("layer_norm", {&x, &w, &b});
     need_gpu({&x, &w, &b});
     if (x.dim() == 0 || x.size(-1) == 0) refuse("layer_norm: x needs a last dimension of at least one channel, got shape ", x.sizes());
     if (x.size(-1) > (1 << 30)) refuse("layer_norm: at most 2^30 channels, got ", x.size(-1));
@@ -223,6 +234,7 @@ struct GroupedLinearFn : torch::autograd::Function<GroupedLinearFn> {
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         no_second_derivative("grouped_linear");
+        no_transforms("grouped_linear", {&grads[0]});
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
         const c10::DeviceGuard guard(x.device());
@@ -268,6 +280,7 @@ Tensor grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& offse
         refuse("grouped_linear: offsets must be int32 or int64 of ", G + 1, " entries, got ", offsets.scalar_type(), " ", offsets.sizes());
     if (bias.defined() && (bias.dim() != 2 || bias.size(0) != G || bias.size(1) != N || !is_real(bias)))
         refuse("grouped_linear: bias must be float32 or bfloat16 of shape (", G, ", ", N, "), got ", bias.scalar_type(), " ", bias.sizes());
+    no_transforms("grouped_linear", {&x, &weight, &bias});
     need_gpu({&x, &weight, &offsets, &bias});
     for (const auto& [name, t] : {std::pair<const char*, const Tensor*>{"weight", &weight}, {"offsets", &offsets}, {"bias", &bias}})
         if (t->defined() && t->device() != x.device()) refuse("grouped_linear: ", name, " is on ", t->device(), ", x on ", x.device());
@@ -295,6 +308,7 @@ Tensor multi_norm(std::vector<Tensor> list, const std::string& what, int kind, b
     std::vector<std::pair<uint64_t, uint64_t>> spans;                         // of the gradients themselves
     for (int i = 0; i < n; ++i) {
         Tensor& t = list[i];
+        no_transforms(what.c_str(), {&t});
         if (t.layout() != at::kStrided) refuse(what, ": gradients must be dense tensors, got ", t.layout());
         if (clip && t.is_inference() && !c10::InferenceMode::is_enabled()) refuse(what, ": a gradient is an inference tensor: it cannot be scaled in place");
         if (!is_real(t)) refuse(what, ": gradients must be float32 or bfloat16 tensors, got ", t.scalar_type());

@@ -13,7 +13,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """(x - mean) / sqrt(var + eps) * weight + bias over the LAST dimension of x (any leading dimensions, any of them zero).
 
     x: fp32 or bf16, on the device; y has its type.  weight, bias: (channels,) of fp32 or bf16 (both of one type), or None.  Gradients of
-    all three; their own gradients are not offered.  The feature maps a `Deeplabv2` returns are logical NCHW: `LayerNorm(c, channel_dim=1)`
+    all three; their own gradients and forward-mode derivatives are not offered.  The feature maps a `Deeplabv2` returns are logical NCHW: `LayerNorm(c, channel_dim=1)`
     normalises their channels without a copy."""
     return _lib.host().layer_norm(x, weight, bias, eps)
 
