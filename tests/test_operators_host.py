@@ -178,3 +178,65 @@ def test_forward_mode_and_traces_are_refused():
     for fn, args in ((layer_norm, (x,)), (lambda a: layer_norm(a, w, b), (x,)), (grouped_linear, (x, gw, off)), (lambda a: get_total_norm([a]), (x,))):
         with pytest.raises(UemError, match="traced"):
             torch.jit.trace(fn, args)
+
+
+def test_sums_over_ranks_are_not_clipped_together_with_other_gradients(monkeypatch):
+    """behind reduce_gradients a model's arena holds sums, until it is cleared, its gradients are dropped or FusedSGD.step has averaged them"""
+    from uemda_amd import dp, optim
+
+    class Model(torch.nn.Linear):
+        def flat_parameters(self):
+            return torch.zeros(8), torch.zeros(8), 8
+    lists = []
+    monkeypatch.setattr(_lib, "host", lambda: type("host", (), {"multi_norm": staticmethod(lambda ps, *a: lists.append(ps) or torch.tensor(1.0))}))
+    monkeypatch.setattr(dp, "world_size", lambda: 2)
+    monkeypatch.setattr(dp.dist, "broadcast", lambda *a, **k: None)
+    monkeypatch.setattr(dp.dist, "all_reduce", lambda *a, **k: None)
+    monkeypatch.setattr(optim, "call", lambda *a: None)
+    monkeypatch.setattr(optim, "stream", lambda: None)
+    m, other, bare = Model(3, 2), torch.ones(2, requires_grad=True), torch.ones(2, requires_grad=True)
+    for i, p in enumerate(m.parameters()):
+        p._uem_owner, p._uem_off = m, 4 * i
+    both = [*m.parameters(), other]
+
+    def gradients():
+        for p in both:
+            p.grad = torch.ones_like(p)
+    gradients()
+    wrap = dp.DataParallel(m, overlap=False)
+    optim.clip_grad_norm_(both, 1.0)
+    assert wrap.reduce_gradients() == 0.5
+    with pytest.raises(UemError, match="sums over ranks"):
+        optim.clip_grad_norm_(both, 1.0)
+    with pytest.raises(UemError, match="sums over ranks"):
+        optim.clip_grad_norm_([other, m.bias], 1.0, float("inf"))
+    optim.clip_grad_norm_([other], 1.0)
+    optim.clip_grad_norm_([m.bias, bare], 1.0)                 # (bare has no gradient: one scale)
+    assert len(lists) == 3
+    optim.FusedSGD(m).step(max_norm=None, grad_prescale=0.5)
+    optim.clip_grad_norm_(both, 1.0)
+    wrap.reduce_gradients()
+    with pytest.raises(UemError, match="sums over ranks"):
+        optim.clip_grad_norm_(both, 1.0)
+    gradients()                                                # new ones, as behind zero_grad(set_to_none=True)
+    optim.clip_grad_norm_(both, 1.0)
+    monkeypatch.setattr(dp, "world_size", lambda: 1)
+    dp.DataParallel(m, overlap=False).reduce_gradients()       # a single rank's sum is its average
+    optim.clip_grad_norm_(both, 1.0)
+    assert len(lists) == 6
+
+
+def test_clearing_a_models_gradients_ends_their_being_sums(monkeypatch):
+    from uemda_amd import dp, optim
+    from uemda_amd.models.Encoder import Deeplabv2
+    monkeypatch.setattr(dp, "world_size", lambda: 2)
+    monkeypatch.setattr(dp.dist, "broadcast", lambda *a, **k: None)
+    monkeypatch.setattr(dp.dist, "all_reduce", lambda *a, **k: None)
+    model = Deeplabv2(dict(backbone=dict(resnet_type="resnet50", output_stride=16, pretrained=False), multi_layer=True, cascade=False, use_ppm=False,
+                           ppm=dict(num_classes=6, use_aux=False, fc_dim=2048), inchannels=2048, num_classes=6, is_ins_norm=True))
+    model._flatten_parameters()
+    model.zero_grad()
+    dp.DataParallel(model, overlap=False).reduce_gradients()
+    assert optim._holds_sums(model)
+    model.zero_grad()
+    assert not optim._holds_sums(model)

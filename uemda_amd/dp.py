@@ -149,7 +149,8 @@ class DataParallel:
             self._trigger_events.clear()
 
     def reduce_gradients(self):
-        """all-reduce(sum) of the gradient arena; returns the prescale (1/world) for FusedSGD.step."""
+        """all-reduce(sum) of the gradient arena; returns the prescale (1/world) for FusedSGD.step.  Gradients outside the arena are not
+        touched: `optim.clip_grad_norm_` refuses to measure such together with the arena's sums."""
         _, garena, _ = self.model.flat_parameters()
         ops.grad_join()            # side-stream / second-stream gradients land before the arena goes out (also after a backward that raised)
         if self._split is not None and self._fwd_calls != self._bwd_calls:
@@ -171,4 +172,6 @@ class DataParallel:
         self._fwd_calls = 0
         self._bwd_calls = 0
         self._trigger_events.clear()
+        # sums, until these gradients are cleared, dropped or stepped with
+        self.model._uem_summed = next((p.grad for p in self.model.parameters() if p.grad is not None), None) if self.world > 1 else None
         return 1.0 / self.world

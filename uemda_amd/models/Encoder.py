@@ -273,6 +273,7 @@ class Deeplabv2(nn.Module):
             return super().zero_grad(set_to_none)
         ops.grad_join()             # weight gradients a failed backward left on the side / second stream must not land after the memset
         self._grad_arena.zero_()
+        self._uem_summed = None
         for p in self.parameters():
             if p.grad is None and p.requires_grad:           # a frozen parameter keeps .grad = None, as under torch autograd
                 p.grad = p._uem_grad_view()

@@ -16,6 +16,12 @@ def _arena_of(params):
     return owner if all(id(p) in listed or not (p.requires_grad or p.grad is not None) for p in owner.parameters()) else None
 
 
+def _holds_sums(model):
+    """does the model's gradient arena hold sums over ranks (DataParallel.reduce_gradients), whose average FusedSGD.step would take?"""
+    summed = getattr(model, "_uem_summed", None)
+    return summed is not None and any(p.grad is summed for p in model.parameters())
+
+
 def grad_norm(model):
     """L2 norm of the flat gradient arena -> 1-element device tensor (two-stage deterministic reduce)."""
     arena, garena, n = model.flat_parameters()
@@ -32,12 +38,21 @@ def _norm_kind(norm_type, what):
     return kind
 
 
+def _tensors(given, what):
+    """a tensor or an iterable of them, as a list"""
+    given = [given] if isinstance(given, torch.Tensor) else list(given)
+    for t in given:
+        if not isinstance(t, torch.Tensor):
+            raise UemError(f"{what}: expected tensors, got {type(t).__name__}")
+    return given
+
+
 def get_total_norm(tensors, norm_type=2.0):
     """The norm over all elements of all `tensors` (a tensor or an iterable; fp32 and bf16 may be mixed), as a 0-dim fp32 device tensor:
     torch.nn.utils.get_total_norm for norm_type 2 or inf.  Squares are summed in 64 bits, in a fixed order; no value is read on the host."""
     what = "get_total_norm"
     ops.grad_join()                # gradients of arena parameters among them may still be on the side / second stream
-    norm = _lib.host().multi_norm([tensors] if isinstance(tensors, torch.Tensor) else list(tensors), what, _norm_kind(norm_type, what), False, None)
+    norm = _lib.host().multi_norm(_tensors(tensors, what), what, _norm_kind(norm_type, what), False, None)
     return torch.tensor(0.0) if norm is None else norm
 
 
@@ -47,15 +62,22 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2):
 
     ALL trained parameters of one uemda_amd model: its flat gradient arena is clipped in one pass.  Any other list -- some of a model's
     parameters, modules outside a model arena, a model together with other modules, fp32 and bf16 mixed -- is clipped tensor by tensor in
-    two passes over the list, and nothing beside it; parameters without a gradient are skipped, gradients that share memory are refused."""
+    two passes over the list, and nothing beside it; parameters without a gradient are skipped, gradients that share memory are refused.
+
+    Behind `DataParallel.reduce_gradients` a model's gradients are SUMS over the ranks (FusedSGD.step takes `max_norm` and the average in one
+    pass), other modules' are whatever the caller made of them: a list of both is refused."""
     what = "clip_grad_norm_"
-    params = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    params = _tensors(parameters, what)
     kind, max_norm = _norm_kind(norm_type, what), float(max_norm)
     if not max_norm >= 0.0:
         raise UemError(f"{what}: max_norm must not be negative, got {max_norm}")
     model = _arena_of(params) if kind == 2 else None
     ops.grad_join()                # weight gradients still on the side / second stream (a backward that raised never ran its join callback)
     if model is None:
+        owners = {id(o): o for o in (getattr(p, "_uem_owner", None) for p in params if not p.is_leaf or p.grad is not None)}
+        if len(owners) > 1 and any(o is not None and _holds_sums(o) for o in owners.values()):
+            raise UemError(f"{what}: the list mixes a model's gradients, which are sums over ranks since reduce_gradients(), with others: clip the "
+                           "model by FusedSGD.step(max_norm=..., grad_prescale=...) and the others by themselves, once they are reduced and averaged")
         norm = _lib.host().multi_norm(params, what, kind, True, max_norm)
         return torch.zeros((), device=params[0].device if params else "cpu") if norm is None else norm
     arena, garena, n = model.flat_parameters()
@@ -116,4 +138,6 @@ class FusedSGD(torch.optim.Optimizer):
                  float(max_norm) if max_norm is not None else 0.0, float(g["lr"]), float(g["momentum"]),
                  float(g["weight_decay"]), 1 if self._steps == 0 else 0, float(grad_prescale), ptr(self.lr_device), stream())
         self._steps += 1
+        if grad_prescale != 1.0:
+            self.model._uem_summed = None      # the kernel has left the average in the arena
         ops.weights_changed()
