@@ -433,7 +433,7 @@ int uem_bn_bwd_apply_bf16(const uint16_t* x, const uint16_t* dy, const uint32_t*
  * ends of the bf16-storage region of the network (max-pool output in, layer4 output out).                             */
 int uem_weight_transpose_bf16(const float* w /* [Cout][KH][KW][Cin] fp32 master */, uint16_t* wt /* [Cin][KH][KW][Cout] bf16 */,
                               int Cout, int KH, int KW, int Cin, void* stream);
-int uem_cast_f32_bf16(const float* x, uint16_t* y, int64_t n, void* stream);
+int uem_cast_f32_bf16(const float* x /* any element */, uint16_t* y /* 8 bytes */, int64_t n, void* stream);
 int uem_cast_bf16_f32(const uint16_t* x, float* y, int64_t n, void* stream);
 
 /* ---- Winograd F(2x2, 3x3) and F(4x4, 3x3) for the stride-1 3x3 convolutions of the deep layers (csrc/winograd.hip) ------

@@ -332,3 +332,21 @@ def test_results_repeat_and_a_captured_step_takes_new_partitions():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(held, want)), o
+
+
+@pytest.mark.parametrize("K,N", [(48, 56), (33, 17), (600, 7)])
+def test_master_weights_that_begin_on_any_element(K, N):
+    """fp32 weights inside a flat parameter buffer, or the weights behind the first group, under bf16 rows: any 4-byte boundary"""
+    o = edges(200, [60, 0, 100], 7)
+    x, w, b, dy = data(200, 3, K, N, torch.bfloat16, 1, wdtype=torch.float32)
+    y0, g0 = check(x, w, b, dy, o)
+    for start in (1, 2, 3, 4):
+        flat = torch.full((start + w.numel() + 5,), float("nan"), device="cuda")
+        v = flat[start:start + w.numel()].view(3, N, K)
+        v.copy_(w)
+        assert v.is_contiguous()
+        y, g = check(x, v, b, dy, o)
+        assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(g, g0))
+    more = torch.cat([torch.full((1, N, K), float("nan"), device="cuda"), w])
+    y, g = check(x, more[1:], b, dy, o)
+    assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(g, g0))
