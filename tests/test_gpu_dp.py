@@ -191,3 +191,34 @@ def test_dropout_masks_differ_between_ranks():
         masks.append(m.cpu())
     assert not torch.equal(masks[0], masks[1])
     assert dropout_seed(1, 0) != dropout_seed(2, 0)
+
+
+def test_a_capture_beside_eager_collectives_of_another_rccl_group(tmp_path):
+    """a group beside the world's (an Aligner's process_group): its eager collectives are off its watchdog's list before its stream is captured"""
+    code = f"""if True:
+        import torch, torch.distributed as dist
+        from uemda_amd.step import retire_collectives
+        torch.cuda.set_device(0)
+        dist.init_process_group("nccl", init_method="file://{tmp_path}/store", rank=0, world_size=1)
+        side = dist.new_group([0])
+        x = torch.ones(1 << 16, device="cuda")
+        for group in (None, side):
+            for _ in range(20):
+                dist.all_reduce(x, group=group)
+        torch.cuda.synchronize()
+        assert retire_collectives()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, capture_error_mode="thread_local"):
+            y = x * 3
+            dist.all_reduce(y, group=side)
+        for k in range(1, 4):
+            x.fill_(k)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert bool((y == 3 * k).all())
+        dist.destroy_process_group()
+        print("CAPTURE_OK", flush=True)
+    """
+    out = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env=dict(os.environ, HSA_ENABLE_IPC_MODE_LEGACY="0"), capture_output=True,
+                         text=True, timeout=120)
+    assert out.returncode == 0 and "CAPTURE_OK" in out.stdout, _report(out.returncode, out.stdout, out.stderr)

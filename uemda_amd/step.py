@@ -252,13 +252,18 @@ def finish(aligner):
 
 
 def retire_collectives():
-    """Waits until the RCCL process group's watchdog has let go of every collective issued so far (a host wait of at most some 100 ms once the
-    device is done with them).  Without such a group: nothing to wait for."""
+    """Waits until the watchdog of every RCCL process group of this process -- the world's, and those that an Aligner or a ClassBalance got as
+    their `process_group` -- has let go of every collective issued so far (a host wait of at most some 100 ms once the device is done with
+    them).  False without such a group.  (torch offers this wait for groups of RCCL alone, not for those that pair it with another backend.)"""
     import torch.distributed as dist
-    if not (dist.is_available() and dist.is_initialized()) or dist.get_backend() != "nccl":
+    if not (dist.is_available() and dist.is_initialized()):
         return False
-    dist.group.WORLD._wait_for_pending_works()
-    return True
+    world = dist.group.WORLD
+    groups = [world] if dist.get_backend() == "nccl" else []
+    groups += [g for g, (backend, _) in list(dist.distributed_c10d._world.pg_map.items()) if g is not world and backend == "nccl"]
+    for g in groups:
+        g._wait_for_pending_works()
+    return bool(groups)
 
 
 class GraphedStep:
