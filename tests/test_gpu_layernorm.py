@@ -320,3 +320,52 @@ def test_a_gradient_with_a_tangent_is_refused():
             with pytest.raises(UemError, match="forward-mode"):
                 torch.autograd.grad(y, x, fa.make_dual(torch.ones_like(y), torch.ones_like(y)), retain_graph=True)
         assert torch.autograd.grad(y, x, torch.ones_like(y))[0].isfinite().all()
+
+
+def close_bounds(x, dy, b, r, D, Dr):
+    """`bounds` where the sums over a row, or over the rows of a column, are kept in 64 bits: D and Dr roundings of half a step, whatever the length"""
+    y, dx, dw, db, hat, rstd, g, w = r
+    ax = x.double().abs().mean(1, keepdim=True) * rstd
+    ehat = U * (D * ax + 2 * D * hat.abs() + D * ax * (hat.abs() + 1) * hat.abs().clamp(max=1))
+    ey = ehat * w.abs() + 2 * U * (y.abs() + (0 if b is None else b.double().abs()))
+    gm, ghm = g.abs().mean(1, keepdim=True), (g * hat).abs().mean(1, keepdim=True)
+    edx = rstd * (U * D * (g.abs() + 2 * gm + 3 * hat.abs() * ghm) + ehat * ghm + hat.abs() * (g.abs() * ehat).mean(1, keepdim=True)) + 2 * D * U * dx.abs()
+    edw = (dy.double().abs() * ehat).sum(0) + U * Dr * (dy.double() * hat).abs().sum(0)
+    return ey, edx, edw, U * Dr * dy.double().abs().sum(0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("c", [8193, 20001, 1000003, 2 ** 24])
+def test_long_rows_keep_their_mean_and_variance(c, dtype):
+    """rows beyond the register kernels, of one value, of values far from zero, of a deviation under the mean's 32-bit sum's error.  Roundings on
+    the way to hat: the mean, the difference, the variance and its sum with eps, the root, the quotient, the product -- 8 with one to spare"""
+    g = torch.Generator(device="cuda").manual_seed(c)
+    rows = torch.tensor([[1.1, 0.0], [100.1, 0.01 if dtype == torch.float32 else 1.0], [-7.3, 0.1]], device="cuda")
+    x = (rows[:, :1] + rows[:, 1:] * torch.randn(3, c, generator=g, device="cuda")).to(dtype)
+    w, b = 1 + 0.2 * torch.randn(c, generator=g, device="cuda"), 0.2 * torch.randn(c, generator=g, device="cuda")
+    dy = (1.1 + 0.1 * torch.randn(3, c, generator=g, device="cuda")).to(dtype)
+    from uemda_amd.norm import layer_norm
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        r = reference(x, w, b, dy, 1e-5)
+        e = close_bounds(x, dy, b, r, 8, 8)
+        for got, want, bound, what in zip((y.detach(), *grads), r, e, ("y", "dx", "dw", "db")):
+            close(got, want, bound, what)
+
+
+def test_parameter_gradients_of_many_rows_that_begin_anywhere():
+    """sums over 260001 rows of one sign by the pass over columns: 64 bits, its blocks' sums rounded once and added in a tree of less than 32"""
+    from uemda_amd.norm import layer_norm
+    rows, c = 260001, 300
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, c + 1, generator=g, device="cuda")[:, 1:]
+    dy = torch.full((rows, c + 1), 1.1, device="cuda")[:, 1:]
+    w, b = torch.ones(c, device="cuda", requires_grad=True), torch.zeros(c, device="cuda", requires_grad=True)
+    grads = torch.autograd.grad(layer_norm(x, w, b), (w, b), dy)
+    with torch.no_grad():
+        r = reference(x, w, b, dy, 1e-5)
+        e = close_bounds(x, dy, b, r, c / 64 + 48, 32)
+        close(grads[0], r[2], e[2], "dw")
+        close(grads[1], r[3], e[3], "db")

@@ -323,26 +323,31 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const LnP p) {
 
 // Any row length, any alignment: a block per row that reads the row again for each sum (rows beyond the register kernels' 8192
 // columns, or rows whose strides and bases share no 16-byte grid).  The parameter gradients are a separate pass over columns.
-template <typename T>
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum_dpp(v);
+// A thread's share has no bound here, so where it is long (A: double) these sums are kept in 64 bits: in 32, the mean of 2^24 elements around 100
+// was off by 0.05, five times their deviation.  A share of up to 32 elements of a row is as good in 32 bits, and the reductions are shorter: 65536 x
+// 513 bf16 that begin anywhere 102 us forward and 175 backward, so 126 and 203 in 64; 4096 x 20001 184 and 320, so 188 and 324.
+template <typename A> __device__ __forceinline__ A block_sum(A v, A* red) {
+    if constexpr (sizeof(A) == 8) v = wave_sum_d(v);
+    else v = wave_sum_dpp(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
-template <typename T>
+__device__ __forceinline__ float mul_add(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double mul_add(double a, double b, double c) { return fma(a, b, c); }
+template <typename T, typename A>
 __global__ __launch_bounds__(256) void layernorm_fwd_any_kernel(const LnP p) {
-    __shared__ float red[4];
-    const float inv = 1.f / (float)p.C;
+    __shared__ A red[4];
+    const A inv = A(1) / (A)p.C;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T* const x = (const T*)p.x + r * p.x_ld;
         T* const y = (T*)p.y + r * p.C;
-        float s = 0.f, q = 0.f;
-        for (int c = threadIdx.x; c < p.C; c += 256) s += Vec<T>::load1(x + c);
-        const float mean = block_sum<T>(s, red) * inv;
-        for (int c = threadIdx.x; c < p.C; c += 256) { const float d = Vec<T>::load1(x + c) - mean; q = fmaf(d, d, q); }
-        const float rstd = 1.f / sqrtf(block_sum<T>(q, red) * inv + p.eps);
+        A s = 0, q = 0;
+        for (int c = threadIdx.x; c < p.C; c += 256) s += (A)Vec<T>::load1(x + c);
+        const float mean = (float)(block_sum<A>(s, red) * inv);
+        for (int c = threadIdx.x; c < p.C; c += 256) { const A d = (A)(Vec<T>::load1(x + c) - mean); q = mul_add(d, d, q); }
+        const float rstd = 1.f / sqrtf((float)(block_sum<A>(q, red) * inv) + p.eps);
         for (int c = threadIdx.x; c < p.C; c += 256) {
             const float ga = p.gamma ? param(p.gamma, p.p16, c) : 1.f, be = p.beta ? param(p.beta, p.p16, c) : 0.f;
             Vec<T>::store1(y + c, fmaf((Vec<T>::load1(x + c) - mean) * rstd, ga, be));
@@ -350,23 +355,22 @@ __global__ __launch_bounds__(256) void layernorm_fwd_any_kernel(const LnP p) {
         if (p.mean != nullptr && threadIdx.x == 0) { p.mean[r] = mean; p.rstd[r] = rstd; }
     }
 }
-template <typename T>
+template <typename T, typename A>
 __global__ __launch_bounds__(256) void layernorm_bwd_any_kernel(const LnP p) {
-    __shared__ float red[4];
-    const float inv = 1.f / (float)p.C;
+    __shared__ A red[4];
+    const A inv = A(1) / (A)p.C;
     for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
         const T* const x = (const T*)p.x + r * p.x_ld;
         const T* const dy = (const T*)p.dy + r * p.dy_ld;
         T* const dx = (T*)p.y + r * p.C;
         const float mean = p.mean[r], rstd = p.rstd[r];
-        float s1 = 0.f, s2 = 0.f;
+        A t1 = 0, t2 = 0;
         for (int c = threadIdx.x; c < p.C; c += 256) {
             const float g = Vec<T>::load1(dy + c) * (p.gamma ? param(p.gamma, p.p16, c) : 1.f);
-            s1 += g;
-            s2 = fmaf(g, (Vec<T>::load1(x + c) - mean) * rstd, s2);
+            t1 += (A)g;
+            t2 = mul_add((A)g, (A)((Vec<T>::load1(x + c) - mean) * rstd), t2);
         }
-        s1 = block_sum<T>(s1, red) * inv;
-        s2 = block_sum<T>(s2, red) * inv;
+        const float s1 = (float)(block_sum<A>(t1, red) * inv), s2 = (float)(block_sum<A>(t2, red) * inv);
         for (int c = threadIdx.x; c < p.C; c += 256) {
             const float g = Vec<T>::load1(dy + c) * (p.gamma ? param(p.gamma, p.p16, c) : 1.f);
             Vec<T>::store1(dx + c, rstd * (g - s1 - (Vec<T>::load1(x + c) - mean) * rstd * s2));
@@ -374,23 +378,23 @@ __global__ __launch_bounds__(256) void layernorm_bwd_any_kernel(const LnP p) {
     }
 }
 // 64 columns x 4 row lanes a block, rows shared out over gridDim.y
-template <typename T>
+template <typename T, typename A>
 __global__ __launch_bounds__(256) void layernorm_cols_kernel(const LnP p) {
-    __shared__ float join[2][4][64];
+    __shared__ A join[2][4][64];
     const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    float a = 0.f, b = 0.f;
+    A a = 0, b = 0;
     if (c < p.C)
         for (int64_t r = (int64_t)blockIdx.y * 4 + w; r < p.rows; r += (int64_t)gridDim.y * 4) {
             const float g = Vec<T>::load1((const T*)p.dy + r * p.dy_ld + c);
-            a = fmaf(g, (Vec<T>::load1((const T*)p.x + r * p.x_ld + c) - p.mean[r]) * p.rstd[r], a);
-            b += g;
+            a = mul_add((A)g, (A)((Vec<T>::load1((const T*)p.x + r * p.x_ld + c) - p.mean[r]) * p.rstd[r]), a);
+            b += (A)g;
         }
     join[0][w][threadIdx.x & 63] = a;
     join[1][w][threadIdx.x & 63] = b;
     __syncthreads();
     if (w < 2 && c < p.C) {
-        const float* const j = &join[w][0][threadIdx.x & 63];
-        p.part[((int64_t)blockIdx.y * 2 + w) * p.C + c] = (j[0] + j[64]) + (j[128] + j[192]);
+        const A* const j = &join[w][0][threadIdx.x & 63];
+        p.part[((int64_t)blockIdx.y * 2 + w) * p.C + c] = (float)((j[0] + j[64]) + (j[128] + j[192]));
     }
 }
 
@@ -527,11 +531,19 @@ int run(LnP p, bool bwd, hipStream_t st) {
         if (W == 4 && v <= 2048) return go<T, 256, W == 4 ? 8 : 4, 1>(p, bwd, st);
     }
     const int nb = p.rows < 256 * 16 ? (int)p.rows : 256 * 16;
-    if (!bwd) { layernorm_fwd_any_kernel<T><<<nb, 256, 0, st>>>(p); return nb; }
-    layernorm_bwd_any_kernel<T><<<nb, 256, 0, st>>>(p);
+    const bool far = p.C > 8192;
+    if (!bwd) {
+        if (far) layernorm_fwd_any_kernel<T, double><<<nb, 256, 0, st>>>(p);
+        else layernorm_fwd_any_kernel<T, float><<<nb, 256, 0, st>>>(p);
+        return nb;
+    }
+    if (far) layernorm_bwd_any_kernel<T, double><<<nb, 256, 0, st>>>(p);
+    else layernorm_bwd_any_kernel<T, float><<<nb, 256, 0, st>>>(p);
     if (p.part == nullptr) return nb;
     const int ny = (int)(uem_cdiv(p.rows, 4) < 64 ? uem_cdiv(p.rows, 4) : 64);
-    layernorm_cols_kernel<T><<<dim3((unsigned)uem_cdiv(p.C, 64), (unsigned)ny), 256, 0, st>>>(p);
+    const dim3 grid((unsigned)uem_cdiv(p.C, 64), (unsigned)ny);
+    if (p.rows > 65536) layernorm_cols_kernel<T, double><<<grid, 256, 0, st>>>(p);       // a thread's share: rows / 256
+    else layernorm_cols_kernel<T, float><<<grid, 256, 0, st>>>(p);
     return ny;
 }
 
