@@ -369,3 +369,19 @@ def test_parameter_gradients_of_many_rows_that_begin_anywhere():
         e = close_bounds(x, dy, b, r, c / 64 + 48, 32)
         close(grads[0], r[2], e[2], "dw")
         close(grads[1], r[3], e[3], "db")
+
+
+def test_rows_of_more_columns_than_a_launch_has_threads_for():
+    """the parameter gradients of 2^25 + 3 columns: 16 columns to a block of 1024 threads would be more than 2^32 threads"""
+    from uemda_amd.norm import layer_norm
+    c = 2 ** 25 + 3
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(2, c, generator=g, device="cuda") for _ in range(2))
+    w, b = (torch.randn(c, generator=g, device="cuda") for _ in range(2))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    with torch.no_grad():
+        r = reference(x, w, b, dy, 1e-5)
+        for got, want, bound, what in zip((y.detach(), *grads), r, close_bounds(x, dy, b, r, 8, 8), ("y", "dx", "dw", "db")):
+            close(got, want, bound, what)

@@ -9,6 +9,8 @@
 // does not depend on timing.
 #include "common.h"
 
+#include <algorithm>
+
 typedef unsigned short bf16_t;
 
 namespace {
@@ -381,20 +383,24 @@ __global__ __launch_bounds__(256) void layernorm_bwd_any_kernel(const LnP p) {
 template <typename T, typename A>
 __global__ __launch_bounds__(256) void layernorm_cols_kernel(const LnP p) {
     __shared__ A join[2][4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
-    A a = 0, b = 0;
-    if (c < p.C)
-        for (int64_t r = (int64_t)blockIdx.y * 4 + w; r < p.rows; r += (int64_t)gridDim.y * 4) {
-            const float g = Vec<T>::load1((const T*)p.dy + r * p.dy_ld + c);
-            a = mul_add((A)g, (A)((Vec<T>::load1((const T*)p.x + r * p.x_ld + c) - p.mean[r]) * p.rstd[r]), a);
-            b += (A)g;
+    const int w = threadIdx.x >> 6;
+    for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < p.C; c0 += (int64_t)gridDim.x * 64) {
+        const int64_t c = c0 + (threadIdx.x & 63);
+        A a = 0, b = 0;
+        if (c < p.C)
+            for (int64_t r = (int64_t)blockIdx.y * 4 + w; r < p.rows; r += (int64_t)gridDim.y * 4) {
+                const float g = Vec<T>::load1((const T*)p.dy + r * p.dy_ld + c);
+                a = mul_add((A)g, (A)((Vec<T>::load1((const T*)p.x + r * p.x_ld + c) - p.mean[r]) * p.rstd[r]), a);
+                b += (A)g;
+            }
+        join[0][w][threadIdx.x & 63] = a;
+        join[1][w][threadIdx.x & 63] = b;
+        __syncthreads();
+        if (w < 2 && c < p.C) {
+            const A* const j = &join[w][0][threadIdx.x & 63];
+            p.part[((int64_t)blockIdx.y * 2 + w) * p.C + c] = (float)((j[0] + j[64]) + (j[128] + j[192]));
         }
-    join[0][w][threadIdx.x & 63] = a;
-    join[1][w][threadIdx.x & 63] = b;
-    __syncthreads();
-    if (w < 2 && c < p.C) {
-        const A* const j = &join[w][0][threadIdx.x & 63];
-        p.part[((int64_t)blockIdx.y * 2 + w) * p.C + c] = (float)((j[0] + j[64]) + (j[128] + j[192]));
+        __syncthreads();
     }
 }
 
@@ -402,26 +408,30 @@ __global__ __launch_bounds__(256) void layernorm_cols_kernel(const LnP p) {
 __global__ __launch_bounds__(1024) void layernorm_params_kernel(const float* __restrict__ part, int nb, int C, void* dgamma, void* dbeta, bool p16) {
     __shared__ float join[64][17];
     const int t = threadIdx.x & 15, sl = threadIdx.x >> 4;
-    const int64_t col = (int64_t)blockIdx.x * 16 + t, n = 2 * (int64_t)C;
-    float s = 0.f;
-    if (col < n) {
+    const int64_t n = 2 * (int64_t)C;
+    for (int64_t c0 = (int64_t)blockIdx.x * 16; c0 < n; c0 += (int64_t)gridDim.x * 16) {
+        const int64_t col = c0 + t;
+        float s = 0.f;
+        if (col < n) {
 #pragma unroll 8
-        for (int b = sl; b < nb; b += 64) s += part[b * n + col];
-    }
-    join[sl][t] = s;
-    __syncthreads();
-    if (sl < 4) {
-        float q = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) q += join[sl * 16 + i][t];
-        q += __shfl_xor(q, 16, 64);
-        q += __shfl_xor(q, 32, 64);
-        void* const out = col < C ? dgamma : dbeta;
-        const int64_t c = col < C ? col : col - C;
-        if (sl == 0 && col < n && out != nullptr) {
-            if (p16) Vec<bf16_t>::store1((bf16_t*)out + c, q);
-            else ((float*)out)[c] = q;
+            for (int b = sl; b < nb; b += 64) s += part[b * n + col];
         }
+        join[sl][t] = s;
+        __syncthreads();
+        if (sl < 4) {
+            float q = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) q += join[sl * 16 + i][t];
+            q += __shfl_xor(q, 16, 64);
+            q += __shfl_xor(q, 32, 64);
+            void* const out = col < C ? dgamma : dbeta;
+            const int64_t c = col < C ? col : col - C;
+            if (sl == 0 && col < n && out != nullptr) {
+                if (p16) Vec<bf16_t>::store1((bf16_t*)out + c, q);
+                else ((float*)out)[c] = q;
+            }
+        }
+        __syncthreads();
     }
 }
 
@@ -431,6 +441,8 @@ int64_t bwd_blocks(int64_t rows) {
     const int64_t n = uem_cdiv(rows < 256 ? rows : rows < 2048 ? 256 : rows / 8, 8) * 8;
     return n > 2048 ? 2048 : n;
 }
+// a launch has fewer than 2^32 threads in a dimension: rows of more columns than so many blocks cover are walked in turns
+constexpr int64_t MOST_BLOCKS = 1 << 20;
 // blocks of a kernel that a CU holds at once (registers): asked for once
 template <typename K> int resident(K kernel) {
     int n = 0;
@@ -541,7 +553,7 @@ int run(LnP p, bool bwd, hipStream_t st) {
     else layernorm_bwd_any_kernel<T, float><<<nb, 256, 0, st>>>(p);
     if (p.part == nullptr) return nb;
     const int ny = (int)(uem_cdiv(p.rows, 4) < 64 ? uem_cdiv(p.rows, 4) : 64);
-    const dim3 grid((unsigned)uem_cdiv(p.C, 64), (unsigned)ny);
+    const dim3 grid((unsigned)std::min<int64_t>(uem_cdiv(p.C, 64), MOST_BLOCKS), (unsigned)ny);
     if (p.rows > 65536) layernorm_cols_kernel<T, double><<<grid, 256, 0, st>>>(p);       // a thread's share: rows / 256
     else layernorm_cols_kernel<T, float><<<grid, 256, 0, st>>>(p);
     return ny;
@@ -580,6 +592,6 @@ extern "C" int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, in
     p.rows = rows; p.x_ld = x_ld; p.dy_ld = dy_ld; p.C = C; p.p16 = (flags & UEM_LN_PARAM_BF16) != 0;
     hipStream_t st = (hipStream_t)stream;
     const int nb = (flags & UEM_LN_BF16) ? run<bf16_t>(p, true, st) : run<float>(p, true, st);
-    if (p.part && nb > 0) layernorm_params_kernel<<<(int)uem_cdiv(2 * (int64_t)C, 16), 1024, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
+    if (p.part && nb > 0) layernorm_params_kernel<<<(int)std::min<int64_t>(uem_cdiv(2 * (int64_t)C, 16), MOST_BLOCKS), 1024, 0, st>>>(p.part, nb, C, dgamma, dbeta, p.p16);
     return uem_check_launch("layernorm_bwd");
 }
