@@ -240,3 +240,13 @@ def test_clearing_a_models_gradients_ends_their_being_sums(monkeypatch):
     assert optim._holds_sums(model)
     model.zero_grad()
     assert not optim._holds_sums(model)
+
+
+def test_more_tiles_than_a_launch_has_threads_for_are_refused():
+    """allowed sizes whose tiles, at 256 or 512 threads each, do not fit the 2^32 threads of a launch: said so before anything is launched"""
+    lib = _lib.load()
+    many, wide = 65535, 65536
+    for flags in (0, 1):
+        assert lib.uem_grouped_fwd(16, 8, 16, 8, None, 16, 16, many, many, 8, wide, flags, None) == -1 and b"2^32 threads" in lib.uem_last_error()
+        assert lib.uem_grouped_dgrad(16, 8, 16, wide, 16, 16, many, many, wide, 8, flags, None) == -1 and b"2^32 threads" in lib.uem_last_error()
+        assert lib.uem_grouped_wgrad(16, wide, 16, 8, 16, 16, 16, 16, many, many, 8, wide, flags, None) == -1 and b"2^32 threads" in lib.uem_last_error()

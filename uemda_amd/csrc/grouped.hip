@@ -774,11 +774,14 @@ __global__ __launch_bounds__(256) void grouped_pad_kernel(const T* __restrict__ 
 }
 
 template <typename T, int FORM, int BM, int BN, int WGM, int WGN>
-void go(const GgP& p, int64_t items, hipStream_t st) {
-    constexpr int LDS = 5 * (BM + BN) * 64;
+int go(const GgP& p, int64_t items, const char* what, hipStream_t st) {
+    constexpr int LDS = 5 * (BM + BN) * 64, THREADS = 64 * WGM * WGN;
+    const int64_t blocks = uem_cdiv(items, 8) * 8;
+    UEM_REQUIRE(blocks * THREADS < ((int64_t)1 << 32), "%s: %lld tiles of %d threads are more than a launch holds (2^32 threads)", what, (long long)items, THREADS);
     auto k = grouped_kernel<T, FORM, BM, BN, WGM, WGN>;
-    if (!uem_allow_lds((const void*)k, LDS)) return;
-    k<<<(unsigned)(uem_cdiv(items, 8) * 8), 64 * WGM * WGN, LDS, st>>>(p);
+    if (!uem_allow_lds((const void*)k, LDS)) return uem_check_launch(what);
+    k<<<(unsigned)blocks, THREADS, LDS, st>>>(p);
+    return uem_check_launch(what);
 }
 
 // Tile of the forward and the data gradient: the one whose slowest CU has the least to do.  The larger a tile the fewer operand bytes a
@@ -845,11 +848,9 @@ int launch_rows(const GgP& p, const char* what, hipStream_t st) {
     }
     const int t = pick_tile(p.T, p.G, width, sizeof(T) == 2);
     const int64_t items = (p.T / TILES[t].bm + (int64_t)(p.G < p.T ? p.G : p.T)) * uem_cdiv(width, TILES[t].bn);   // at most so many tiles: one of each group with rows is not full
-    UEM_REQUIRE(items < ((int64_t)1 << 31), "%s: %lld tiles are more than the kernels count", what, (long long)items);
-    if (sizeof(T) == 2 && t == 0) go<bf16_t, FORM, 256, 256, 2, 4>(p, items, st);
-    else if (t == 1) go<T, FORM, 128, 128, 2, 2>(p, items, st);
-    else go<T, FORM, 64, 128, 1, 4>(p, items, st);
-    return uem_check_launch(what);
+    if (sizeof(T) == 2 && t == 0) return go<bf16_t, FORM, 256, 256, 2, 4>(p, items, what, st);
+    if (t == 1) return go<T, FORM, 128, 128, 2, 2>(p, items, what, st);
+    return go<T, FORM, 64, 128, 1, 4>(p, items, what, st);
 }
 
 template <int FORM>
@@ -931,13 +932,14 @@ extern "C" int uem_grouped_wgrad(const void* dy, int dy_ld, const void* x, int x
     p.chunk = wgrad_chunk(T, G, N, K, bm);
     const int64_t slots = wgrad_slots(T, p.chunk), items = (T / p.chunk + (int64_t)G) * uem_cdiv(N, bm) * uem_cdiv(K, bm);
     UEM_REQUIRE(slots == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "grouped_wgrad: no workspace, or not on a 16-byte boundary");
-    UEM_REQUIRE(items < ((int64_t)1 << 31), "grouped_wgrad: %lld tiles are more than the kernels count", (long long)items);
     p.db = db;
     p.part = workspace;
     p.part_db = workspace + (slots * (int64_t)N * K + 3) / 4 * 4;
-    if (bm == 256) go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, st);
-    else if (h) go<bf16_t, WGRAD, 128, 128, 2, 2>(p, items, st);
-    else go<float, WGRAD, 128, 128, 2, 2>(p, items, st);
+    const char* const what = "grouped_wgrad";
+    const int launched = bm == 256 ? go<bf16_t, WGRAD, 256, 256, 2, 4>(p, items, what, st)
+                         : h       ? go<bf16_t, WGRAD, 128, 128, 2, 2>(p, items, what, st)
+                                   : go<float, WGRAD, 128, 128, 2, 2>(p, items, what, st);
+    if (launched != UEM_OK) return launched;
     if (slots > 0) {
         const int64_t chunks = uem_cdiv(T, p.chunk), nb = uem_cdiv((int64_t)N * K, chunks > 64 ? 64 : chunks > 16 ? 256 : 1024);
         const int64_t most = slots / 2 < G ? slots / 2 : G;                    // groups of several chunks

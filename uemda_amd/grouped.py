@@ -19,7 +19,8 @@ def grouped_linear(x, weight, offsets, bias=None):
     bf16 for the product, their gradient comes back in fp32).  bias: (groups, out) fp32 or bf16, or None.  offsets: (groups + 1,) int32 or
     int64 on the device, not decreasing; it is not read on the host: an entry below an earlier one counts as that one, entries beyond the
     rows as the number of rows.  Rows in front of offsets[0] and behind offsets[-1] belong to no group: y is zero there, as their gradient
-    is, and what they hold (even NaN) reaches no weight's gradient.  Sums run in 32 bits and in a fixed order."""
+    is, and what they hold (even NaN) reaches no weight's gradient.  Sums run in 32 bits and in a fixed order.
+    Refused: 2^30 rows or 2^16 groups and more, more than 2^20 channels, more tiles than a launch holds (some ten million)."""
     return _lib.host().grouped_linear(x, weight, offsets, bias)
 
 
