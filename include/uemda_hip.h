@@ -520,6 +520,8 @@ int uem_layernorm_bwd(const void* x, int64_t x_ld, const void* dy, int64_t dy_ld
 #define UEM_GROUPED_OFFSETS_64 8
 int uem_grouped_pad(const void* src, int64_t src_ld, void* dst, int dst_ld, int cols, int64_t rows, int flags, void* stream);
 int uem_grouped_any_rows(int T, int G, int K, int N, int flags, int dgrad);
+/* rows of the tile that a call of these sizes is cut into (wgrad: rows of W): form 0 fwd, 1 dgrad, 2 wgrad -> 32 (few rows), 64, 128 or 256 */
+int uem_grouped_tile_rows(int T, int G, int K, int N, int flags, int form);
 int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void* bias, void* y, const void* offsets, int T, int G, int K, int N,
                     int flags, void* stream);
 int uem_grouped_dgrad(const void* dy, int dy_ld, const void* w, int w_ld, void* dx, const void* offsets, int T, int G, int K, int N, int flags,

@@ -350,3 +350,46 @@ def test_master_weights_that_begin_on_any_element(K, N):
     more = torch.cat([torch.full((1, N, K), float("nan"), device="cuda"), w])
     y, g = check(x, more[1:], b, dy, o)
     assert torch.equal(y, y0) and all(torch.equal(p, q) for p, q in zip(g, g0))
+
+
+# T, K, N, lengths, rows in front; which of forward, data gradient, weight gradient run on tiles of 256 x 256 (the library is asked, so that a
+# change of its rules cannot empty this).  A stage is 32 of the reduction: 1000 makes 32 stages (even), 776 and 777 make 25, 1001 makes 32
+# with a ragged last one; the dominating groups are several chunks and a rest, whose partial sums are joined
+LARGE = [
+    (25000, 1000, 1000, [14001, 0, 5000, 3003, 1], 900, "fdw"),
+    (28000, 776, 1000, [300, 20000, 257, 0, 5000], 31, "fdw"),
+    (28000, 777, 1001, [0, 25111, 1, 255, 700], 1000, "fdw"),       # odd widths: padded copies, results element by element
+    (28000, 1001, 777, [28000, 0, 0, 0, 0], 0, "fdw"),               # one group of all rows
+    (28000, 1000, 1000, [0, 0, 0, 0, 0], 13, "fdw"),                 # no row has a group
+    (30000, 1023, 1021, [5000, 5001, 4999, 5000, 5000, 4000], 500, "fdw"),
+    (40000, 520, 1000, [39000, 1, 2, 3, 4, 500], 200, "fd"),
+] + [(25000, k, 1000, [9000, 3, 0, 12000, 77], 5, "f") for k in (8, 33, 72, 104, 136, 168)] \
+  + [(25000, 1000, n, [9000, 3, 0, 12000, 77], 5, "d") for n in (8, 33, 72, 104, 136, 168)]     # 1 to 6 stages: fewer than, as many as and more than the ring
+
+
+@pytest.mark.parametrize("T,K,N,lens,head,forms", LARGE)
+def test_tiles_of_256(T, K, N, lens, head, forms):
+    from uemda_amd import _lib
+    for form in forms:
+        assert _lib.load().uem_grouped_tile_rows(T, len(lens), K, N, 1, "fdw".index(form)) == 256, form
+    x, w, b, dy = data(T, len(lens), K, N, torch.bfloat16, T + K + N)
+    o = edges(T, lens, head)
+    x[:o[0]], dy[:o[0]], x[o[-1]:], dy[o[-1]:] = float("nan"), float("inf"), float("inf"), float("nan")      # rows of no group
+    check(x, w, b, dy, o)
+
+
+def test_tiles_of_256_repeat_to_the_bit():
+    """both waves of a SIMD, the ring and the join in a fixed order: ten steps of the same operands, others between them"""
+    from uemda_amd.grouped import grouped_linear
+    T, K, N, lens = 28000, 776, 1000, [300, 20000, 257, 0, 5000]
+    x, w, b, dy = data(T, 5, K, N, torch.bfloat16, 0)
+    off = torch.tensor(edges(T, lens, 31), device="cuda")
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def once():
+        y = grouped_linear(*leaves[:2], off, leaves[2])
+        return y, *torch.autograd.grad(y, leaves, dy)
+    want = once()
+    for _ in range(9):
+        grouped_linear(dy.detach(), w.detach().transpose(1, 2), off)
+        assert all(torch.equal(p, q) for p, q in zip(once(), want))

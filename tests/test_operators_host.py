@@ -250,3 +250,12 @@ def test_more_tiles_than_a_launch_has_threads_for_are_refused():
         assert lib.uem_grouped_fwd(16, 8, 16, 8, None, 16, 16, many, many, 8, wide, flags, None) == -1 and b"2^32 threads" in lib.uem_last_error()
         assert lib.uem_grouped_dgrad(16, 8, 16, wide, 16, 16, many, many, wide, 8, flags, None) == -1 and b"2^32 threads" in lib.uem_last_error()
         assert lib.uem_grouped_wgrad(16, wide, 16, 8, 16, 16, 16, 16, many, many, 8, wide, flags, None) == -1 and b"2^32 threads" in lib.uem_last_error()
+
+
+def test_the_tile_that_sizes_are_cut_into():
+    lib = _lib.load()
+    assert [lib.uem_grouped_tile_rows(32768, 7, 2048, 512, 1, form) for form in range(3)] == [128, 256, 256]
+    assert lib.uem_grouped_tile_rows(9, 6, 2048, 512, 1, 0) == 32 and lib.uem_grouped_tile_rows(9, 6, 512, 2048, 1, 1) == 32      # few rows, long reductions
+    assert lib.uem_grouped_tile_rows(9, 6, 2048, 512, 1, 1) == 64      # 256 tiles of 32 x 32 are too many for a reduction of 512
+    for args in ((0, 1, 8, 8, 1, 0), (8, 1, 8, 8, 1, 3), (8, 1, 8, 8, 1, -1)):
+        assert lib.uem_grouped_tile_rows(*args) == -1

@@ -152,6 +152,7 @@ SIGNATURES = {
     "uem_multi_clip": [P, P, P, I, I, P, P, F, P],
     "uem_grouped_pad": [P, L, P, I, I, L, I, P],
     "uem_grouped_any_rows": [I, I, I, I, I, I],
+    "uem_grouped_tile_rows": [I, I, I, I, I, I],
     "uem_grouped_fwd": [P, I, P, I, P, P, P, I, I, I, I, I, P],
     "uem_grouped_dgrad": [P, I, P, I, P, P, I, I, I, I, I, P],
     "uem_grouped_wgrad_workspace_floats": [I, I, I, I, I],

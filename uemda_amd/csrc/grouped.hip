@@ -897,6 +897,13 @@ extern "C" int uem_grouped_any_rows(int T, int G, int K, int N, int flags, int d
     const bool is16 = (flags & UEM_GROUPED_BF16) != 0;
     return dgrad ? takes_few<DGRAD>(T, G, K, N, is16) : takes_few<FWD>(T, G, K, N, is16);
 }
+extern "C" int uem_grouped_tile_rows(int T, int G, int K, int N, int flags, int form) {
+    const bool is16 = (flags & UEM_GROUPED_BF16) != 0;
+    UEM_REQUIRE(T > 0 && G > 0 && K > 0 && N > 0 && form >= FWD && form <= WGRAD, "grouped_tile_rows: bad arguments");
+    if (form == WGRAD) return wgrad_tile(T, N, K, is16);
+    if (form == FWD ? takes_few<FWD>(T, G, K, N, is16) : takes_few<DGRAD>(T, G, K, N, is16)) return 32;
+    return TILES[pick_tile(T, G, form == FWD ? N : K, is16)].bm;
+}
 extern "C" int uem_grouped_fwd(const void* x, int x_ld, const void* w, int w_ld, const void* bias, void* y, const void* offsets, int T, int G, int K,
                                int N, int flags, void* stream) {
     const int rc = check<FWD>(x, w, y, offsets, T, G, K, N, x_ld, w_ld, flags, "grouped_fwd");
