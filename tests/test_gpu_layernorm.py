@@ -385,3 +385,27 @@ def test_rows_of_more_columns_than_a_launch_has_threads_for():
         r = reference(x, w, b, dy, 1e-5)
         for got, want, bound, what in zip((y.detach(), *grads), r, close_bounds(x, dy, b, r, 8, 8), ("y", "dx", "dw", "db")):
             close(got, want, bound, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_map_without_one_row_stride_is_copied_once(dtype):
+    """contiguous NCHW through channel_dim = 1: the forward's copy is what the backward pass reads, so that it takes memory for dx alone (and the
+    parameter gradients' sums, less than a quarter of a map here); and the gradient is that of the values that went in"""
+    from uemda_amd.norm import LayerNorm
+    g = torch.Generator().manual_seed(2)
+    ln = LayerNorm(64, channel_dim=1).cuda()
+    x = torch.randn(4, 64, 96, 100, generator=g).to(dtype).cuda()
+    dy = torch.randn(4, 64, 96, 100, generator=g).to(dtype).cuda().contiguous(memory_format=torch.channels_last)
+    ref = [t.clone() for t in torch.autograd.grad(ln(x.clone().contiguous(memory_format=torch.channels_last).requires_grad_()), list(ln.parameters()), dy)]
+    leaf = x.clone().requires_grad_()
+    into = leaf * 1
+    y = ln(into)
+    with torch.no_grad():
+        into.mul_(float("nan"))                                                # (the node holds the copy: this is allowed, and changes nothing)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    dx, *grads = torch.autograd.grad(y, [into, *ln.parameters()], dy)
+    peak = torch.cuda.max_memory_allocated() - before
+    assert peak < 1.25 * x.numel() * x.element_size(), peak / (x.numel() * x.element_size())
+    assert all(torch.equal(p, q) for p, q in zip(grads, ref)) and dx.isfinite().all()

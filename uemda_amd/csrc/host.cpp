@@ -104,7 +104,7 @@ void no_outside_graph(const char* what, std::initializer_list<const Tensor*> lis
 std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 
 // ---- layer norm ------------------------------------------------------------------------------------------------------------------------
-// t as rows of c channels: itself where one row stride describes it, a copy otherwise
+// t as rows of c channels: itself where it is dense, or 2-d with a stride between its rows; a copy otherwise
 Tensor norm_rows(const Tensor& t, int64_t c, int64_t& ld) {
     if (t.is_contiguous()) { ld = c; return t; }
     if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= c) { ld = t.stride(0); return t; }
@@ -112,27 +112,28 @@ Tensor norm_rows(const Tensor& t, int64_t c, int64_t& ld) {
     return t.contiguous();
 }
 int norm_flags(const Tensor& x, bool param16) { return (is16(x) ? UEM_LN_BF16 : 0) | (param16 ? UEM_LN_PARAM_BF16 : 0); }
-std::pair<Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool save) {
+struct Normed { Tensor y, stats, x; };             // x: as the kernel reads it
+Normed norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, double eps, bool save) {
     const c10::DeviceGuard guard(x.device());
     const int64_t c = x.size(-1), rows = x.numel() / c;
     Tensor y = at::empty(x.sizes(), x.options()), stats;
     if (save) stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
-    if (rows == 0) return {y, stats};
+    if (rows == 0) return {y, stats, x};
     int64_t ld;
     const Tensor xr = norm_rows(x, c, ld);
     float* const mean = save ? stats.data_ptr<float>() : nullptr;
     CALL(uem_layernorm_fwd, ptr(xr), ld, ptr(w), ptr(b), mptr(y), mean, save ? mean + rows : nullptr, rows, (int)c, (float)eps,
          norm_flags(x, is16(w) || is16(b)), stream_of(x));
-    return {y, stats};
+    return {y, stats, xr};
 }
 struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& w_, const std::optional<Tensor>& b_, double eps) {
         const Tensor w = w_.value_or(Tensor()), b = b_.value_or(Tensor());
-        auto [y, stats] = norm_forward(x, w, b, eps, true);
-        ctx->save_for_backward({x, w, stats});
+        const Normed r = norm_forward(x, w, b, eps, true);
+        ctx->save_for_backward({r.x, w, r.stats});
         ctx->saved_data["param16"] = is16(w) || is16(b);
         ctx->saved_data["bias"] = b.defined();
-        return y;
+        return r.y;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
         no_second_derivative("layer_norm");
@@ -180,7 +181,7 @@ Tensor layer_norm(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
         no_outside_graph("layer_norm", {&x, &w, &b});
         return LayerNormFn::apply(x, maybe(w), maybe(b), eps);
     }
-    return norm_forward(x, w, b, eps, false).first;
+    return norm_forward(x, w, b, eps, false).y;
 }
 
 // ---- grouped products -------------------------------------------------------------------------------------------------------------------

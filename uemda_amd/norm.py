@@ -20,7 +20,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 class LayerNorm(nn.Module):
     """`layer_norm` with its parameters.  channel_dim: -1 (rows of channels, NHWC maps) or 1 (logical NCHW maps; channels_last memory is
-    used as it is, anything else is copied once)."""
+    used as it is, anything else is copied once, and that copy is what the backward pass reads)."""
 
     def __init__(self, channels, eps=1e-5, affine=True, bias=True, channel_dim=-1):
         super().__init__()
