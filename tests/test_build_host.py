@@ -1,0 +1,25 @@
+"""What `make` would run, on the CPU: nothing is compiled here."""
+import os
+import subprocess
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "uemda_amd", "csrc")
+
+
+def commands(*args):
+    res = subprocess.run(["make", "-n", "-C", CSRC, *args], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr
+    return res.stdout
+
+
+def test_the_c_library_alone_needs_neither_torch_nor_python():
+    out = commands("-B", "PY=/nonexistent/python3")
+    assert "libuemda_hip.so" in out and "grouped.hip" in out and "_host.so" not in out
+    assert "_host.so" in commands("-B", "host") and "-ltorch_python" in commands("-B", "host")
+
+
+def test_build_makes_both(monkeypatch):
+    from uemda_amd import _lib
+    seen = []
+    monkeypatch.setattr(_lib.subprocess, "run", lambda cmd, **kw: seen.append(cmd) or type("done", (), {"returncode": 0, "stdout": "", "stderr": ""}))
+    assert _lib.build() == _lib.LIB_PATH
+    assert "all" in seen[0] and "host" in seen[0]

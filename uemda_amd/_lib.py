@@ -6,6 +6,7 @@ caller gets an exception.  Nothing here imports `oracle/`.
 import ctypes
 import os
 import subprocess
+import sys
 from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int64, c_uint64, c_void_p
 
 import torch  # noqa: F401  -- MUST precede dlopen: torch brings its own libamdhip64.so.7; loading ours first
@@ -184,14 +185,14 @@ class UemError(RuntimeError):
 
 
 def build(verbose=False):
-    """Compile every HIP source for gfx950 into uemda_amd/libuemda_hip.so (hipcc cross-compiles)."""
-    cmd = ["make", "-C", os.path.join(_HERE, "csrc"), "-j", str(min(8, os.cpu_count() or 1))]
+    """Compile every HIP source for gfx950 into uemda_amd/libuemda_hip.so (hipcc cross-compiles), and the host extension uemda_amd/_host.so."""
+    cmd = ["make", "-C", os.path.join(_HERE, "csrc"), "all", "host", f"PY={sys.executable}", "-j", str(min(8, os.cpu_count() or 1))]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or res.returncode != 0:
         print(res.stdout[-4000:])
         print(res.stderr[-4000:])
     if res.returncode != 0:
-        raise UemError("hipcc build of libuemda_hip.so failed")
+        raise UemError("the build of libuemda_hip.so and _host.so failed")
     return LIB_PATH
 
 
