@@ -23,3 +23,11 @@ def test_build_makes_both(monkeypatch):
     monkeypatch.setattr(_lib.subprocess, "run", lambda cmd, **kw: seen.append(cmd) or type("done", (), {"returncode": 0, "stdout": "", "stderr": ""}))
     assert _lib.build() == _lib.LIB_PATH
     assert "all" in seen[0] and "host" in seen[0]
+
+
+def test_objects_follow_the_flags_they_are_built_with():
+    """a Makefile with other flags (the one that left packed fp32 arithmetic out) makes every object anew, not those alone whose sources changed"""
+    sources = [f for f in os.listdir(CSRC) if f.endswith((".hip", ".cpp")) and f != "host.cpp"]
+    out = commands("-W", "Makefile")
+    assert all(f" -c {f} " in out for f in sources) and "-packed-fp32-ops" in out, out
+    assert "host.cpp" in commands("-W", "Makefile", "host")
