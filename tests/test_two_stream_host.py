@@ -76,3 +76,15 @@ def test_shadow_running_statistics_swap_and_restore():
     # state_dict round trip: the views are ordinary buffers
     sd = m.state_dict()
     assert sd["encoder.resnet.layer1.0.bn1.running_mean"].data_ptr() == real_mean.data_ptr()
+
+
+def test_the_priority_switches_say_that_they_are_gone():
+    import os
+    import subprocess
+    import sys
+    code = "import warnings\nwith warnings.catch_warnings(record=True) as w:\n    warnings.simplefilter('always')\n    import uemda_amd.ops\nprint([str(x.message) for x in w if 'PRIORITY' in str(x.message)])"
+    for env, said in (({}, 0), ({"UEM_SECOND_PRIORITY": "0"}, 0), ({"UEM_SECOND_PRIORITY": "-1"}, 1), ({"UEM_SIDE_PRIORITY": "-1", "UEM_SECOND_PRIORITY": "-1"}, 2)):
+        base = {k: v for k, v in os.environ.items() if "PRIORITY" not in k}
+        out = subprocess.run([sys.executable, "-c", code], env={**base, **env}, capture_output=True, text=True,
+                             cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+        assert out.returncode == 0 and out.stdout.count("no effect any more") == said, (env, out.stdout, out.stderr)

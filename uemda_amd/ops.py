@@ -4,6 +4,7 @@ device allocations and the stream; every arithmetic step is a `uem_*` HIP kernel
 Internal activation layout is NHWC: tensors of shape (N, H, W, C), contiguous, fp32.
 """
 import ctypes
+import warnings
 import weakref
 
 import torch
@@ -186,6 +187,10 @@ SIDE_HOLD = os.environ.get("UEM_SIDE_HOLD", "1") != "0"       # 0: record_stream
 # Every stream here has the default priority: work on streams of different priorities has hung on this hardware for good.  (With the
 # second graph's stream at high priority its chain and the first one ended together: bf16 36.5-36.7 -> 35.7-35.8 ms, fp32 98.7-99.9 ->
 # 98.5-98.6 ms a step -- not worth a hang.)
+for _name in ("UEM_SIDE_PRIORITY", "UEM_SECOND_PRIORITY"):
+    if os.environ.get(_name, "0") not in ("", "0"):
+        warnings.warn(f"{_name} has no effect any more: every stream has the default priority (streams of different priorities have hung on this hardware)",
+                      RuntimeWarning, stacklevel=2)
 
 
 class _Side:
