@@ -259,3 +259,32 @@ def test_some_of_a_models_parameters_are_clipped_alone():
     coef = torch.clamp(32.0 / (alone + 1e-6), max=1.0)
     for b, p in zip(before, params):
         assert torch.equal(p.grad, b * coef)
+
+
+@pytest.mark.parametrize("kind", [2, INF])
+@pytest.mark.parametrize("bad", [float("nan"), INF])
+def test_a_norm_that_is_not_finite_raises_where_it_is_asked_to(kind, bad):
+    """the signature of torch's two functions; nothing is scaled by a call that raises"""
+    from uemda_amd import UemError
+    from uemda_amd.models.Encoder import Deeplabv2
+    from uemda_amd.optim import clip_grad_norm_, get_total_norm
+    t, u = torch.full((5000,), 3.0).cuda(), torch.ones(33, dtype=torch.bfloat16).cuda()
+    assert torch.equal(clip_grad_norm_(params_of([t.clone(), u.clone()]), 1.0, kind, True, foreach=False), get_total_norm([t, u], kind, error_if_nonfinite=True))
+    assert float(clip_grad_norm_([], 1.0, error_if_nonfinite=True)) == float(get_total_norm([], error_if_nonfinite=True, foreach=True)) == 0.0
+    t[77] = bad
+    keep = [t.clone(), u.clone()]
+    with pytest.raises(UemError, match="total norm is"):
+        get_total_norm([t, u], kind, error_if_nonfinite=True)
+    with pytest.raises(UemError, match="total norm is"):
+        clip_grad_norm_(params_of([t, u]), 1.0, kind, error_if_nonfinite=True)
+    assert torch.equal(t.nan_to_num(7.0), keep[0].nan_to_num(7.0)) and torch.equal(u, keep[1])
+    model = Deeplabv2(dict(backbone=dict(resnet_type="resnet50", output_stride=16, pretrained=False), multi_layer=True, cascade=False, use_ppm=False,
+                           ppm=dict(num_classes=6, use_aux=False, fc_dim=2048), inchannels=2048, num_classes=6, is_ins_norm=True)).cuda()
+    model.zero_grad()
+    params = list(model.parameters())
+    for p in params:
+        p.grad.fill_(2.0)
+    params[3].grad.view(-1)[0] = bad
+    with pytest.raises(UemError, match="total norm is"):
+        clip_grad_norm_(params, 1.0, kind, error_if_nonfinite=True)
+    assert all(bool((p.grad == 2.0).all()) for p in params[4:])

@@ -47,18 +47,28 @@ def _tensors(given, what):
     return given
 
 
-def get_total_norm(tensors, norm_type=2.0):
+def _finite(norm, what):
+    if not bool(torch.isfinite(norm)):
+        raise UemError(f"{what}: the total norm is {float(norm)}, so nothing is scaled (error_if_nonfinite=False would let it through)")
+
+
+def get_total_norm(tensors, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """The norm over all elements of all `tensors` (a tensor or an iterable; fp32 and bf16 may be mixed), as a 0-dim fp32 device tensor:
-    torch.nn.utils.get_total_norm for norm_type 2 or inf.  Squares are summed in 64 bits, in a fixed order; no value is read on the host."""
+    torch.nn.utils.get_total_norm for norm_type 2 or inf.  Squares are summed in 64 bits, in a fixed order.  error_if_nonfinite reads the norm on
+    the host and raises where it is infinite or none (otherwise no value is read there); `foreach` chooses nothing: there is one way."""
     what = "get_total_norm"
     ops.grad_join()                # gradients of arena parameters among them may still be on the side / second stream
     norm = _lib.host().multi_norm(_tensors(tensors, what), what, _norm_kind(norm_type, what), False, None)
-    return torch.tensor(0.0) if norm is None else norm
+    norm = torch.tensor(0.0) if norm is None else norm
+    if error_if_nonfinite:
+        _finite(norm, what)
+    return norm
 
 
-def clip_grad_norm_(parameters, max_norm, norm_type=2):
+def clip_grad_norm_(parameters, max_norm, norm_type=2, error_if_nonfinite=False, foreach=None):
     """Drop-in for torch.nn.utils.clip_grad_norm_: scales the gradients of `parameters` (a tensor or an iterable) in place by
-    min(max_norm / (norm + 1e-6), 1) and returns their total norm, a device scalar; norm_type is 2 or inf.
+    min(max_norm / (norm + 1e-6), 1) and returns their total norm, a device scalar; norm_type is 2 or inf.  error_if_nonfinite reads the norm
+    on the host and raises, with nothing scaled, where it is infinite or none; `foreach` chooses nothing: there is one way.
 
     ALL trained parameters of one uemda_amd model: its flat gradient arena is clipped in one pass.  Any other list -- some of a model's
     parameters, modules outside a model arena, a model together with other modules, fp32 and bf16 mixed -- is clipped tensor by tensor in
@@ -78,10 +88,16 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2):
         if len(owners) > 1 and any(o is not None and _holds_sums(o) for o in owners.values()):
             raise UemError(f"{what}: the list mixes a model's gradients, which are sums over ranks since reduce_gradients(), with others: clip the "
                            "model by FusedSGD.step(max_norm=..., grad_prescale=...) and the others by themselves, once they are reduced and averaged")
+        if error_if_nonfinite:
+            norm = _lib.host().multi_norm(params, what, kind, True, None)
+            if norm is not None:
+                _finite(norm, what)
         norm = _lib.host().multi_norm(params, what, kind, True, max_norm)
         return torch.zeros((), device=params[0].device if params else "cpu") if norm is None else norm
     arena, garena, n = model.flat_parameters()
     norm = grad_norm(model)
+    if error_if_nonfinite:
+        _finite(norm, what)
     coef = torch.clamp(max_norm / (norm + 1e-6), max=1.0)      # one scalar
     call("uem_scale_by_scalar", ptr(garena), None, n, ptr(coef), stream())
     return norm[0]
