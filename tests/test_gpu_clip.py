@@ -288,3 +288,23 @@ def test_a_norm_that_is_not_finite_raises_where_it_is_asked_to(kind, bad):
     with pytest.raises(UemError, match="total norm is"):
         clip_grad_norm_(params, 1.0, kind, error_if_nonfinite=True)
     assert all(bool((p.grad == 2.0).all()) for p in params[4:])
+
+
+def test_slots_of_parameters_without_a_gradient_do_not_count():
+    """behind torch's zero_grad(set_to_none=True) the arena still holds the pass before: what no later pass has written is no gradient"""
+    from uemda_amd.models.Encoder import Deeplabv2
+    from uemda_amd.optim import clip_grad_norm_
+    model = Deeplabv2(dict(backbone=dict(resnet_type="resnet50", output_stride=16, pretrained=False), multi_layer=True, cascade=False, use_ppm=False,
+                           ppm=dict(num_classes=6, use_aux=False, fc_dim=2048), inchannels=2048, num_classes=6, is_ins_norm=True)).cuda()
+    model.zero_grad()
+    params = list(model.parameters())
+    for p in params:
+        p.grad.fill_(1.0)
+    for p in params[40:]:
+        p.grad = None
+    want = exact_norm([p.grad for p in params[:40]], 2)
+    got = clip_grad_norm_(params, 1.0)
+    assert abs(float(got) - want) <= 2.0 ** -23 * want
+    assert all(p.grad is None for p in params[40:])
+    for p in params[:40]:
+        assert ((p.grad.double() - 1 / (want + 1e-6)).abs() <= 5 * 2.0 ** -24 / want).all()

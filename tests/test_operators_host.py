@@ -259,3 +259,24 @@ def test_the_tile_that_sizes_are_cut_into():
     assert lib.uem_grouped_tile_rows(9, 6, 2048, 512, 1, 1) == 64      # 256 tiles of 32 x 32 are too many for a reduction of 512
     for args in ((0, 1, 8, 8, 1, 0), (8, 1, 8, 8, 1, 3), (8, 1, 8, 8, 1, -1)):
         assert lib.uem_grouped_tile_rows(*args) == -1
+
+
+def test_a_models_arena_is_its_gradients_only_where_they_are_its_slots():
+    """a parameter without a gradient, or with a tensor of the caller's, leaves its slot of the arena with something else in it"""
+    from uemda_amd import optim
+    from uemda_amd.models.Encoder import Deeplabv2
+    model = Deeplabv2(dict(backbone=dict(resnet_type="resnet50", output_stride=16, pretrained=False), multi_layer=True, cascade=False, use_ppm=False,
+                           ppm=dict(num_classes=6, use_aux=False, fc_dim=2048), inchannels=2048, num_classes=6, is_ins_norm=True))
+    model._flatten_parameters()
+    params = list(model.parameters())
+    assert optim._arena_of(params) is None                     # no gradient yet
+    model.zero_grad()
+    assert optim._arena_of(params) is model and optim._arena_of(params[1:]) is None
+    slot, params[5].grad = params[5].grad, None
+    assert optim._arena_of(params) is None
+    params[5].grad = torch.zeros_like(params[5])
+    assert optim._arena_of(params) is None
+    params[5].grad = slot
+    params[9].requires_grad_(False)
+    params[9].grad = None
+    assert optim._arena_of(params) is model and optim._arena_of([p for p in params if p.requires_grad]) is model

@@ -7,13 +7,19 @@ from .ops import UemError, call, ptr, stream
 
 
 def _arena_of(params):
-    """the model whose flat gradient arena IS the gradients of `params`: all of them are its parameters, and none that it trains or that
-    has a gradient is missing (frozen ones may be, as in `filter(lambda p: p.requires_grad, model.parameters())`).  Else None"""
+    """the model whose flat gradient arena IS the gradients of `params`: all of them are its parameters, each has its slot of the arena as its
+    gradient (not None, as behind torch's zero_grad(set_to_none=True), whose slots hold what an earlier pass left, and no tensor of the
+    caller's), and none that it trains or that has a gradient is missing (frozen ones may be, as in
+    `filter(lambda p: p.requires_grad, model.parameters())`).  Else None"""
     owner = getattr(params[0], "_uem_owner", None) if params else None
     if owner is None or any(getattr(p, "_uem_owner", None) is not owner for p in params):
         return None
     listed = {id(p) for p in params}
-    return owner if all(id(p) in listed or not (p.requires_grad or p.grad is not None) for p in owner.parameters()) else None
+    if not all(id(p) in listed or not (p.requires_grad or p.grad is not None) for p in owner.parameters()):
+        return None
+    base = owner.flat_parameters()[1].data_ptr()
+    attached = (p.grad is not None and p.grad.data_ptr() == base + 4 * p._uem_off or not p.requires_grad and p.grad is None for p in params)
+    return owner if all(attached) else None
 
 
 def _holds_sums(model):
