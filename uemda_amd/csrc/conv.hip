@@ -2732,7 +2732,8 @@ static bool conv_bf16_areg_try(const ConvP& p, unsigned xb, unsigned wb, hipStre
     if (p.Cin != 64 && p.Cin != 128 && p.Cin != 256) return false;
     if (p.x_ld % 8 != 0 || p.y_ld % 8 != 0 || (((uintptr_t)p.x | (uintptr_t)p.y) & 15) != 0) return false;
     // plain products only: the residual tails and the BatchNorm-backward partial sums of a data gradient stay with conv_bf16_kernel (their
-    // forms in this kernel were 20-64 % slower than its epilogue, and one of them raced)
+    // forms in this kernel were 20-64 % slower than its epilogue, and one of them gave wrong elements that changed from run to run, for a
+    // cause that was not found: they are gone)
     if (p.accumulate || (MODE == 1 && p.tile_bnbwd != nullptr)) return false;
     const int npanels = p.M / 512;
     // Rule (scripts/sweep_conv_bf16_ring.py SWEEP=areg, profiles/r06_m_conv_bf16_areg_sweep_*.txt; forced on = wherever legal): a reduction
