@@ -31,3 +31,22 @@ def test_objects_follow_the_flags_they_are_built_with():
     out = commands("-W", "Makefile")
     assert all(f" -c {f} " in out for f in sources) and "-packed-fp32-ops" in out, out
     assert "host.cpp" in commands("-W", "Makefile", "host")
+
+
+def test_loads_in_inline_asm_wait_in_their_own_block():
+    """the compiler takes an asm's outputs as written where it stands: a load whose wait stands in a later statement can be copied, or its
+    register given away, while it is in flight"""
+    import re
+    load = re.compile(r"\b(ds_read|ds_load|global_load|buffer_load|flat_load|scratch_load|s_load|s_buffer_load)\w*")
+    seen = 0
+    for name in sorted(os.listdir(CSRC)):
+        if not name.endswith((".hip", ".h", ".cpp")):
+            continue
+        text = open(os.path.join(CSRC, name)).read()
+        for m in re.finditer(r"\basm\s*(volatile)?\s*\(", text):
+            strings = re.match(r'(\s*"(?:[^"\\]|\\.)*")+', text[m.end():])
+            body = strings.group(0) if strings else ""
+            if load.search(body):
+                seen += 1
+                assert "s_waitcnt" in body, (name, text.count("\n", 0, m.start()) + 1, body[:80])
+    assert seen >= 4

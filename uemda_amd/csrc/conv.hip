@@ -539,6 +539,26 @@ __global__ __launch_bounds__(256, NBUF == 1 ? 3 : 2) void conv_fwd_kernel(const 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) unsigned int* lds_u32p;
 typedef float f32x4v __attribute__((ext_vector_type(4)));
+// N 16-byte LDS reads of a lane, STEP bytes apart (PAIR: two neighbours every STEP), issued together and waited for in the SAME block: to the compiler
+// an asm's outputs are written where it stands, so reads whose wait stood in a later statement could be copied or overwritten while in flight
+template <int N, int STEP, bool PAIR> __device__ __forceinline__ void lds_rows(unsigned at, f32x4v (&v)[N]) {
+    static_assert(N == 2 || N == 4 || N == 8, "a block of its own for each");
+#define LDS_AT(i) "n"(PAIR ? (i) / 2 * STEP + (i) % 2 * 16 : (i) * STEP)
+    if constexpr (N == 2)
+        asm volatile("ds_read_b128 %0, %2 offset:%3\n\tds_read_b128 %1, %2 offset:%4\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]) : "v"(at), LDS_AT(0), LDS_AT(1) : "memory");
+    else if constexpr (N == 4)
+        asm volatile("ds_read_b128 %0, %4 offset:%5\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %4 offset:%7\n\tds_read_b128 %3, %4 offset:%8\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(at), LDS_AT(0), LDS_AT(1), LDS_AT(2), LDS_AT(3) : "memory");
+    else
+        asm volatile("ds_read_b128 %0, %8 offset:%9\n\tds_read_b128 %1, %8 offset:%10\n\tds_read_b128 %2, %8 offset:%11\n\tds_read_b128 %3, %8 offset:%12\n\t"
+                     "ds_read_b128 %4, %8 offset:%13\n\tds_read_b128 %5, %8 offset:%14\n\tds_read_b128 %6, %8 offset:%15\n\tds_read_b128 %7, %8 offset:%16\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]), "=&v"(v[4]), "=&v"(v[5]), "=&v"(v[6]), "=&v"(v[7])
+                     : "v"(at), LDS_AT(0), LDS_AT(1), LDS_AT(2), LDS_AT(3), LDS_AT(4), LDS_AT(5), LDS_AT(6), LDS_AT(7) : "memory");
+#undef LDS_AT
+}
 typedef unsigned u32x4v __attribute__((ext_vector_type(4)));
 extern "C" __device__ void uem_raw_buffer_load_lds(i32x4 rsrc, lds_u32p lds, int size, int voffset, int soffset, int offset,
                                                    int aux) __asm("llvm.amdgcn.raw.buffer.load.lds");
@@ -1256,14 +1276,9 @@ __global__ __launch_bounds__(2 * BMT, BMT == 128 ? 2 : 1) void conv_bf16_kernel(
             // every outstanding LDS-DMA piece AND, with them, behind the previous chunk's global stores (an `s_waitcnt vmcnt(0)` in front
             // of each chunk's first read, found in the ISA: the next tile's operand prefetch and the write acknowledgements of the rows
             // just stored were waited for four times per tile); the reads are ordered by the barrier above and waited for right here
-            f32x4v svlo[NRP], svhi[NRP];
+            f32x4v sv[2 * NRP];
             if constexpr (RAWB) {
-#pragma unroll
-                for (int u = 0; u < NRP; ++u) {
-                    const unsigned la = (unsigned)(unsigned long long)(lds_u32p)(&stg[(srow + u * RPP) * LDW + sc8]);
-                    asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %2 offset:16" : "=&v"(svlo[u]), "=&v"(svhi[u]) : "v"(la));
-                }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                lds_rows<2 * NRP, RPP * LDW * 4, true>((unsigned)(unsigned long long)(lds_u32p)(&stg[srow * LDW + sc8]), sv);
                 __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
@@ -1273,7 +1288,7 @@ __global__ __launch_bounds__(2 * BMT, BMT == 128 ? 2 : 1) void conv_bf16_kernel(
                 float v[8];
                 if constexpr (RAWB) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) { v[e] = svlo[u][e]; v[4 + e] = svhi[u][e]; }
+                    for (int e = 0; e < 4; ++e) { v[e] = sv[2 * u][e]; v[4 + e] = sv[2 * u + 1][e]; }
                 } else {
                     *reinterpret_cast<float4*>(&v[0]) = *reinterpret_cast<const float4*>(&stg[row * LDW + sc8]);
                     *reinterpret_cast<float4*>(&v[4]) = *reinterpret_cast<const float4*>(&stg[row * LDW + sc8 + 4]);
@@ -2397,20 +2412,17 @@ __global__ __launch_bounds__(512, 1) void pw_bf16_stream_kernel(const PwP p, con
     auto trickle = [&](int nsend) {
         while (nsend > 0 && tr_left > 0) {
             f32x4v v[4];
-            unsigned go[4];
-            int nb = 0;
+            unsigned go[4], la[4];
+            const int nb = min(min(nsend, tr_left), 4);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (u < nsend && tr_left > 0) {
-                    const int c = (NSL - tr_left) * 256 + stid, row = c >> 4, ch = c & 15;
-                    const unsigned la = (unsigned)(unsigned long long)(lds_u32p)(ob + row * PBN + ch * 8);
-                    asm volatile("ds_read_b128 %0, %1" : "=v"(v[u]) : "v"(la));
-                    go[u] = (unsigned)(pm0 + row) * (unsigned)p.ldc + (unsigned)(pn0 + ch * 8);
-                    --tr_left;
-                    nb = u + 1;
-                }
+            for (int u = 0; u < 4; ++u) {                                      // slices past the last one read it again
+                const int c = (NSL - tr_left + min(u, nb - 1)) * 256 + stid, row = c >> 4, ch = c & 15;
+                la[u] = (unsigned)(unsigned long long)(lds_u32p)(ob + row * PBN + ch * 8);
+                go[u] = (unsigned)(pm0 + row) * (unsigned)p.ldc + (unsigned)(pn0 + ch * 8);
             }
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            tr_left -= nb;
+            asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %6\n\tds_read_b128 %3, %7\n\ts_waitcnt lgkmcnt(0)"
+                         : "=&v"(v[0]), "=&v"(v[1]), "=&v"(v[2]), "=&v"(v[3]) : "v"(la[0]), "v"(la[1]), "v"(la[2]), "v"(la[3]) : "memory");
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int u = 0; u < 4; ++u)
@@ -2685,12 +2697,7 @@ __global__ __launch_bounds__(512, 1) void pw_bf16_areg_kernel(const PwP p, const
             __builtin_amdgcn_sched_barrier(0);
             {
                 f32x4v v[NSTR];
-#pragma unroll
-                for (int u = 0; u < NSTR; ++u) {
-                    const unsigned la = (unsigned)(unsigned long long)(lds_u32p)(ow + (u * 8 + (lane >> 3)) * 64 + (lane & 7) * 8);
-                    asm volatile("ds_read_b128 %0, %1" : "=v"(v[u]) : "v"(la));
-                }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                lds_rows<NSTR, 8 * 64 * 2, false>((unsigned)(unsigned long long)(lds_u32p)(ow + (lane >> 3) * 64 + (lane & 7) * 8), v);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int u = 0; u < NSTR; ++u)
